@@ -388,6 +388,86 @@ int ody_dequant_fp8_e5m2(const void* q, int64_t n, float* out);   /* from_bf8 (t
 int ody_dequant_fp16(const void* q, int64_t n, float* out);   /* the exact FP16 -> float32 upcast */
 int ody_dequant_bf16(const void* q, int64_t n, float* out);   /* the exact BF16 -> float32 upcast */
 
+/* ---- the linear layer over the step's quantised weights ------------------
+ * What reads the 4-bit weights that the step (or ody_quantize) leaves, and
+ * what makes the gradients it takes (extensions; the reference's linear
+ * layer works on float tensors):
+ *
+ *   ody_fp4_linear        y[m, n]  = s sum_k x[m, k] W[n, k]
+ *   ody_fp4_linear_dgrad  dx[m, k] = s sum_n dy[m, n] W[n, k]
+ *   ody_linear_wgrad8     dw[n, k] = alpha sum_m dy[m, n] x'[m, k] (+ add[n, k])
+ *
+ * W is the [out_features, in_features] weight in the bytes of kind
+ * ODY_Q_MXFP4, _NVFP4, _NVFP4_TENSOR or _MXFP4_OCP, exactly as
+ * ody_get_quant and ody_quantize lay it out (blocks of the flattened tensor;
+ * one may straddle two rows), any alignment.  x' is an activation kept in 8
+ * bits (below).  Operands and results are float32, float16 or bfloat16, any
+ * combination.  Every product is exact; sums are taken in float32 in an
+ * order that depends on the shapes only (same call, same bits), and each
+ * result is rounded once.  Non-finite inputs, and blocks with a non-finite
+ * scale, make the results they reach non-finite.
+ *
+ * The plain forms take contiguous buffers in host or device memory and
+ * return when done.  The _on_stream forms take memory of the current GPU
+ * only, add row pitches in elements (lda, ldo >= the columns) and a scalar
+ * alpha, enqueue their kernels on `stream` and return (capturable; no
+ * allocation, no synchronisation): the caller keeps the buffers until the
+ * work is done, and gives every call that may overlap another one a
+ * workspace of its own, 256-byte aligned, of at least
+ * ody_linear_workspace(op, ...) bytes (may be 0).  tensor_scale (a device
+ * float, or NULL for 1) is ODY_Q_NVFP4_TENSOR's; results are multiplied by
+ * alpha * *tensor_scale.  Outputs must not overlap inputs, except that add
+ * may be dw itself (accumulation in place). */
+#define ODY_LINEAR_FORWARD 0
+#define ODY_LINEAR_DGRAD 1
+#define ODY_LINEAR_WGRAD 2
+/* workspace bytes of one call (-1: bad arguments); act_dtype is x's or dy's */
+int64_t ody_linear_workspace(int32_t op, int64_t rows, int64_t out_features, int64_t in_features, int32_t act_dtype);
+int ody_fp4_linear_on_stream(int32_t kind, const void* q, const float* tensor_scale, float alpha,
+                             int64_t out_features, int64_t in_features, const void* x, int32_t x_dtype, int64_t rows,
+                             int64_t ldx, void* y, int32_t y_dtype, int64_t ldy, void* workspace,
+                             size_t workspace_bytes, void* stream);
+int ody_fp4_linear_dgrad_on_stream(int32_t kind, const void* q, const float* tensor_scale, float alpha,
+                                   int64_t out_features, int64_t in_features, const void* dy, int32_t dy_dtype,
+                                   int64_t rows, int64_t lddy, void* dx, int32_t dx_dtype, int64_t lddx,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+int ody_fp4_linear(int32_t kind, const void* q, float tensor_scale, int64_t out_features, int64_t in_features,
+                   const void* x, int32_t x_dtype, int64_t rows, void* y, int32_t y_dtype);
+int ody_fp4_linear_dgrad(int32_t kind, const void* q, float tensor_scale, int64_t out_features, int64_t in_features,
+                         const void* dy, int32_t dy_dtype, int64_t rows, void* dx, int32_t dx_dtype);
+
+/* Activations kept in 8 bits between the forward and the backward pass.  Per
+ * row and 32 columns one power of two 2^X, the least with amax <= largest *
+ * 2^X over the finite elements (X clamped to -117..119 for E4M3, -110..112
+ * for E5M2), stored as the byte X + 127; codes are x / 2^X rounded to nearest
+ * even, saturating only where X is clamped.  NaN stays NaN; an infinity stays
+ * one in E5M2 and becomes NaN in E4M3, which has none, so the gradients made
+ * from it still fail the step's finite check.  codes: rows of
+ * ody_act8_groups(cols) * 32 bytes, 16-byte aligned, zeros behind the last
+ * column; scales: rows of ody_act8_groups(cols) bytes.  Restored values are
+ * exact in float32 and bfloat16; in float16 they are rounded, and finite ones
+ * stay within its range. */
+#define ODY_A8_E4M3 0
+#define ODY_A8_E5M2 1
+int64_t ody_act8_groups(int64_t cols);
+int ody_act8_save_on_stream(int32_t format, const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx,
+                            uint8_t* codes, uint8_t* scales, void* stream);
+int ody_act8_load_on_stream(int32_t format, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols,
+                            void* out, int32_t dtype, int64_t ldo, void* stream);
+int ody_act8_save(int32_t format, const void* x, int32_t dtype, int64_t rows, int64_t cols, uint8_t* codes,
+                  uint8_t* scales);
+int ody_act8_load(int32_t format, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* out,
+                  int32_t dtype);
+/* The weight gradient from a saved activation: dy [rows, out_features], dw
+ * and add (or NULL) contiguous [out_features, in_features] of dw_dtype. */
+int ody_linear_wgrad8_on_stream(int32_t format, const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                                int64_t in_features, const void* dy, int32_t dy_dtype, int64_t out_features,
+                                int64_t lddy, float alpha, const void* add, void* dw, int32_t dw_dtype,
+                                void* workspace, size_t workspace_bytes, void* stream);
+int ody_linear_wgrad8(int32_t format, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t in_features,
+                      const void* dy, int32_t dy_dtype, int64_t out_features, float alpha, const void* add, void* dw,
+                      int32_t dw_dtype);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,8 @@ F32, F16, BF16 = 0, 1, 2
 SGD, ADAM, ADAMW, LION, RMSPROP, ADAGRAD = 0, 1, 2, 3, 4, 5
 (Q_NONE, Q_FP16, Q_BF16, Q_FP8_E4M3, Q_FP8_E5M2, Q_FP8_E4M3_TENSOR, Q_MXFP4, Q_NVFP4,
  Q_NVFP4_TENSOR, Q_MXFP4_OCP) = range(10)
+A8_E4M3, A8_E5M2 = 0, 1
+LINEAR_FORWARD, LINEAR_DGRAD, LINEAR_WGRAD = 0, 1, 2
 BUF_MASTER, BUF_STATE1, BUF_STATE2, BUF_GRAD, BUF_DP_GRAD = range(5)
 
 QUANT_NAMES = {
@@ -125,6 +127,21 @@ _SIGS = {
     "ody_adagrad_step": (C.c_int, [_p, _p, _p, _i64] + [C.c_double] * 3 + [_p, _p]),
     "ody_quantize": (C.c_int, [_i32, _p, _i32, _i64, _p, _p]),
     "ody_dequantize": (C.c_int, [_i32, _p, _i64, C.c_float, _p]),
+    "ody_linear_workspace": (_i64, [_i32, _i64, _i64, _i64, _i32]),
+    "ody_fp4_linear_on_stream": (C.c_int, [_i32, _p, _p, C.c_float, _i64, _i64, _p, _i32, _i64, _i64, _p, _i32, _i64,
+                                           _p, C.c_size_t, _p]),
+    "ody_fp4_linear_dgrad_on_stream": (C.c_int, [_i32, _p, _p, C.c_float, _i64, _i64, _p, _i32, _i64, _i64, _p, _i32,
+                                                 _i64, _p, C.c_size_t, _p]),
+    "ody_fp4_linear": (C.c_int, [_i32, _p, C.c_float, _i64, _i64, _p, _i32, _i64, _p, _i32]),
+    "ody_fp4_linear_dgrad": (C.c_int, [_i32, _p, C.c_float, _i64, _i64, _p, _i32, _i64, _p, _i32]),
+    "ody_act8_groups": (_i64, [_i64]),
+    "ody_act8_save_on_stream": (C.c_int, [_i32, _p, _i32, _i64, _i64, _i64, _p, _p, _p]),
+    "ody_act8_load_on_stream": (C.c_int, [_i32, _p, _p, _i64, _i64, _p, _i32, _i64, _p]),
+    "ody_act8_save": (C.c_int, [_i32, _p, _i32, _i64, _i64, _p, _p]),
+    "ody_act8_load": (C.c_int, [_i32, _p, _p, _i64, _i64, _p, _i32]),
+    "ody_linear_wgrad8_on_stream": (C.c_int, [_i32, _p, _p, _i64, _i64, _p, _i32, _i64, _i64, C.c_float, _p, _p, _i32,
+                                              _p, C.c_size_t, _p]),
+    "ody_linear_wgrad8": (C.c_int, [_i32, _p, _p, _i64, _i64, _p, _i32, _i64, C.c_float, _p, _p, _i32]),
 }
 EXPORTED = tuple(_SIGS)
 

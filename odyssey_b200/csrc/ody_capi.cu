@@ -13,23 +13,12 @@
 #include <vector>
 
 #include "../../include/odyssey_mp.h"
+#include "ody_host.h"
 #include "ody_internal.h"
 
 using namespace ody;
 
 static thread_local std::string g_err;
-
-static int fail(int code, const std::string& msg) {
-  g_err = msg;
-  return code;
-}
-
-#define ODY_CUDA(call)                                                              \
-  do {                                                                              \
-    cudaError_t e_ = (call);                                                        \
-    if (e_ != cudaSuccess)                                                          \
-      return fail(ODY_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_)); \
-  } while (0)
 
 // ---------------------------------------------------------------------------
 // NCCL, bound at run time (dlopen) so that a process which already loaded a
@@ -189,15 +178,12 @@ static cudaError_t timing_collect(ody_ctx* c, int64_t slot) {
   return cudaSuccess;
 }
 
-static bool is_device_ptr(const void* p);  // device memory of the current GPU, or managed
 
 static int ctx_fail(ody_ctx* c, int code, const std::string& msg) {
   g_err = msg;
   if (c) c->err = msg;
   return code;
 }
-
-static size_t dtype_size(int gdt) { return gdt == DT_F32 ? 4 : 2; }
 
 extern "C" int ody_abi_version(void) { return ODY_ABI_VERSION; }
 
@@ -1472,95 +1458,6 @@ extern "C" void ody_ctx_destroy(ody_ctx* c) {
 // host operands are staged through temporary device buffers on the calling
 // thread's default stream.
 // ---------------------------------------------------------------------------
-// Device memory usable by this call's kernels: managed memory, or device
-// memory of the calling thread's current GPU.  Another GPU's memory is not
-// (without peer access a kernel reading it faults): device_elsewhere() names
-// that case so the caller can refuse it before any launch.
-static int device_of(const void* p) {
-  if (!p) return -1;
-  cudaPointerAttributes a;
-  if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
-    cudaGetLastError();
-    return -1;
-  }
-  if (a.type == cudaMemoryTypeManaged) return INT32_MAX;  // reachable from every GPU
-  return a.type == cudaMemoryTypeDevice ? a.device : -1;
-}
-
-static bool is_device_ptr(const void* p) {
-  const int d = device_of(p);
-  if (d < 0) return false;
-  if (d == INT32_MAX) return true;
-  int cur = 0;
-  cudaGetDevice(&cur);
-  return d == cur;
-}
-
-static bool device_elsewhere(const void* p) {
-  const int d = device_of(p);
-  return d >= 0 && d != INT32_MAX && !is_device_ptr(p);
-}
-
-namespace {
-struct Staged {
-  void* user = nullptr;
-  void* dev = nullptr;
-  size_t bytes = 0;
-  bool owned = false;
-};
-
-struct Scope {
-  cudaStream_t st = cudaStreamPerThread;
-  std::vector<Staged> bufs;
-  ~Scope() {
-    for (auto& b : bufs)
-      if (b.owned && b.dev) cudaFreeAsync(b.dev, st);
-  }
-  // in: copy host data to device; out-only: allocate
-  cudaError_t stage(const void* user, size_t bytes, bool copy_in, void** dev) {
-    if (!user) {
-      *dev = nullptr;
-      return cudaSuccess;
-    }
-    if (device_elsewhere(user)) return cudaErrorInvalidDevice;
-    if (is_device_ptr(user)) {
-      *dev = const_cast<void*>(user);
-      bufs.push_back({const_cast<void*>(user), *dev, bytes, false});
-      return cudaSuccess;
-    }
-    void* d = nullptr;
-    cudaError_t e = cudaMallocAsync(&d, bytes < 16 ? 16 : bytes, st);
-    if (e != cudaSuccess) return e;
-    if (copy_in) {
-      e = cudaMemcpyAsync(d, user, bytes, cudaMemcpyHostToDevice, st);
-      if (e != cudaSuccess) return e;
-    }
-    bufs.push_back({const_cast<void*>(user), d, bytes, true});
-    *dev = d;
-    return cudaSuccess;
-  }
-  cudaError_t copy_out(void* user) {
-    for (auto& b : bufs)
-      if (b.user == user && b.owned) return cudaMemcpyAsync(user, b.dev, b.bytes, cudaMemcpyDeviceToHost, st);
-    return cudaSuccess;
-  }
-};
-}  // namespace
-
-#define ODY_STAGE(S, ptr, bytes, in, dev)                                             \
-  do {                                                                                \
-    cudaError_t se_ = (S).stage((ptr), (bytes), (in), (void**)(dev));                 \
-    if (se_ == cudaErrorInvalidDevice)                                                \
-      return fail(ODY_ERR_ARG, "a buffer is device memory of another GPU than the current one"); \
-    if (se_ != cudaSuccess)                                                           \
-      return fail(ODY_ERR_CUDA, std::string("staging a buffer: ") + cudaGetErrorString(se_)); \
-  } while (0)
-
-static int check_dtype(int dt) {
-  if (dt < DT_F32 || dt > DT_BF16) return fail(ODY_ERR_DTYPE, "unsupported dtype " + std::to_string(dt));
-  return ODY_OK;
-}
-
 static void current_device_tables() {
   int dev = 0;
   cudaGetDevice(&dev);

@@ -1,0 +1,275 @@
+// ody_linear_capi.cu -- C entry points of the quantised linear layer
+// (include/odyssey_mp.h): argument checks, staging for host callers, and the
+// launches of ody_linear.cu.
+#include <exception>
+
+#include "ody_host.h"
+#include "ody_linear.h"
+
+using namespace ody;
+
+namespace {
+
+constexpr int64_t kMaxDim = INT32_MAX - 1024;  // of rows, features and (with padding) row pitches
+
+// no C++ exception leaves a C entry point
+template <class F>
+int guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return fail(ODY_ERR_STATE, std::string("host error: ") + e.what());
+  }
+}
+
+int check_shape(int64_t rows, int64_t out, int64_t in) {
+  if (rows <= 0 || out <= 0 || in <= 0) return fail(ODY_ERR_SHAPE, "linear: rows and features must be positive");
+  if (rows > kMaxDim || out > kMaxDim || in > kMaxDim) return fail(ODY_ERR_SHAPE, "linear: a dimension is too large");
+  return ODY_OK;
+}
+
+int check_pitch(int64_t ld, int64_t cols, const char* what) {
+  if (ld < cols || ld > ((int64_t)1 << 38))
+    return fail(ODY_ERR_SHAPE, std::string("the row pitch of ") + what + " is smaller than its columns, or too large");
+  return ODY_OK;
+}
+
+bool is_w4(int kind) {
+  return kind == ODY_Q_MXFP4 || kind == ODY_Q_NVFP4 || kind == ODY_Q_NVFP4_TENSOR || kind == ODY_Q_MXFP4_OCP;
+}
+
+// what both forms of a product check, and its arguments for the launcher
+int product(LinearArgs& a, int op, int32_t kind, int64_t rows, int64_t out, int64_t in, const void* act, int32_t adt,
+            int64_t lda, const void* q, const void* scales, void* c, int32_t cdt, int64_t ldc) {
+  if (op == LIN_WGRAD ? (kind != ODY_A8_E4M3 && kind != ODY_A8_E5M2) : !is_w4(kind))
+    return fail(ODY_ERR_ARG, op == LIN_WGRAD ? "unknown 8-bit activation format " + std::to_string(kind)
+                                             : "the weight must be one of the 4-bit kinds, not " + std::to_string(kind));
+  if (check_dtype(adt) || check_dtype(cdt)) return ODY_ERR_DTYPE;
+  if (int rc = check_shape(rows, out, in)) return rc;
+  if (int rc = check_pitch(lda, op == LIN_FORWARD ? in : out, op == LIN_FORWARD ? "x" : "dy")) return rc;
+  if (int rc = check_pitch(ldc, op == LIN_FORWARD ? out : in, op == LIN_FORWARD ? "y" : (op == LIN_DGRAD ? "dx" : "dw")))
+    return rc;
+  if (!act || !q || !c || (op == LIN_WGRAD && !scales)) return fail(ODY_ERR_ARG, "null pointer");
+  a = LinearArgs{};
+  a.op = op;
+  a.rows = rows, a.out = out, a.in = in;
+  a.a = act, a.a_dtype = adt, a.lda = lda;
+  a.kind = kind;
+  a.q = (const uint8_t*)q, a.scales = (const uint8_t*)scales;
+  a.o.c = c, a.o.dtype = cdt, a.o.ld = ldc;
+  a.o.alpha = 1.0f;
+  return ODY_OK;
+}
+
+int aligned_to(const void* p, int dtype, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) % dtype_size(dtype))
+    return fail(ODY_ERR_ARG, std::string(what) + " is not aligned to its element type");
+  return ODY_OK;
+}
+
+int launch(const LinearArgs& a, void* ws, size_t ws_bytes, cudaStream_t st) {
+  if (aligned_to(a.a, a.a_dtype, "an operand") || aligned_to(a.o.c, a.o.dtype, "the output") ||
+      (a.o.add && aligned_to(a.o.add, a.o.dtype, "add")))
+    return ODY_ERR_ARG;
+  ODY_CUDA(launch_linear(a, ws, ws_bytes, st));
+  return ODY_OK;
+}
+
+int on_stream(const LinearArgs& a, void* ws, size_t ws_bytes, void* stream, const char* name) {
+  const int64_t need = linear_workspace(a);
+  if (need > 0 && (!ws || (int64_t)ws_bytes < need))
+    return fail(ODY_ERR_ARG, std::string(name) + ": needs " + std::to_string(need) + " bytes of workspace");
+  if (!is_device_ptr(a.a) || !is_device_ptr(a.q) || (a.scales && !is_device_ptr(a.scales)) || !is_device_ptr(a.o.c) ||
+      (a.o.tscale && !is_device_ptr(a.o.tscale)) || (a.o.add && !is_device_ptr(a.o.add)) ||
+      (need > 0 && !is_device_ptr(ws)))
+    return fail(ODY_ERR_ARG, std::string(name) + " takes memory of the current GPU only");
+  if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 255u))
+    return fail(ODY_ERR_ARG, std::string(name) + ": the workspace must be 256-byte aligned");
+  return launch(a, ws, ws_bytes, (cudaStream_t)stream);
+}
+
+// host or device buffers, contiguous; waits for the result
+int staged(LinearArgs a, float alpha) {
+  const int64_t asz = a.rows * a.lda * (int64_t)dtype_size(a.a_dtype);
+  const int64_t crows = a.op == LIN_WGRAD ? a.out : a.rows;
+  const int64_t csz = crows * a.o.ld * (int64_t)dtype_size(a.o.dtype);
+  const int64_t groups = (a.in + kA8Group - 1) / kA8Group;
+  const int64_t qsz = a.op == LIN_WGRAD ? a.rows * groups * kA8Group : ody_quant_bytes(a.kind, a.out * a.in);
+  a.o.alpha = alpha;
+  Scope S;
+  S.bufs.reserve(8);
+  void *da, *dq, *dc, *ds = nullptr, *dadd = nullptr, *ws = nullptr;
+  void* const c = a.o.c;
+  ODY_STAGE(S, a.a, (size_t)asz, true, &da);
+  ODY_STAGE(S, a.q, (size_t)qsz, true, &dq);
+  if (a.scales) ODY_STAGE(S, a.scales, (size_t)(a.rows * groups), true, &ds);
+  if (a.o.add && a.o.add != c) ODY_STAGE(S, a.o.add, (size_t)csz, true, &dadd);
+  ODY_STAGE(S, c, (size_t)csz, a.o.add == c, &dc);
+  if (a.o.add == c) dadd = dc;
+  const int64_t need = linear_workspace(a);
+  if (need > 0) {
+    ODY_CUDA(cudaMallocAsync(&ws, (size_t)need, S.st));
+    S.bufs.push_back({nullptr, ws, 0, true});
+  }
+  a.a = da, a.q = (const uint8_t*)dq, a.scales = (const uint8_t*)ds, a.o.c = dc, a.o.add = dadd;
+  if (int rc = launch(a, ws, (size_t)need, S.st)) return rc;
+  ODY_CUDA(S.copy_out(c));
+  ODY_CUDA(cudaStreamSynchronize(S.st));
+  return ODY_OK;
+}
+
+int act8_args(int32_t fmt, const void* x, int32_t dt, int64_t rows, int64_t cols, int64_t ld, const void* codes,
+              const void* scales) {
+  if (fmt != ODY_A8_E4M3 && fmt != ODY_A8_E5M2)
+    return fail(ODY_ERR_ARG, "unknown 8-bit activation format " + std::to_string(fmt));
+  if (check_dtype(dt)) return ODY_ERR_DTYPE;
+  if (rows <= 0 || cols <= 0) return fail(ODY_ERR_SHAPE, "cannot save an empty activation");
+  if (rows > kMaxDim || cols > kMaxDim) return fail(ODY_ERR_SHAPE, "linear: a dimension is too large");
+  if (int rc = check_pitch(ld, cols, "the activation")) return rc;
+  if (!x || !codes || !scales) return fail(ODY_ERR_ARG, "null pointer");
+  return ODY_OK;
+}
+
+int act8_device(const void* x, int32_t dt, const void* codes, const void* scales, const char* name) {
+  if (!is_device_ptr(x) || !is_device_ptr(codes) || !is_device_ptr(scales))
+    return fail(ODY_ERR_ARG, std::string(name) + " takes memory of the current GPU only");
+  if (reinterpret_cast<uintptr_t>(codes) & 15u)
+    return fail(ODY_ERR_ARG, std::string(name) + ": codes must be 16-byte aligned");
+  return aligned_to(x, dt, "the activation");
+}
+
+}  // namespace
+
+extern "C" int64_t ody_act8_groups(int64_t cols) { return cols > 0 ? (cols + kA8Group - 1) / kA8Group : 0; }
+
+extern "C" int ody_act8_save_on_stream(int32_t fmt, const void* x, int32_t dt, int64_t rows, int64_t cols, int64_t ldx,
+                                       uint8_t* codes, uint8_t* scales, void* stream) {
+  return guarded([&]() -> int {
+    if (int rc = act8_args(fmt, x, dt, rows, cols, ldx, codes, scales)) return rc;
+    if (int rc = act8_device(x, dt, codes, scales, "ody_act8_save_on_stream")) return rc;
+    ODY_CUDA(launch_act8_save(fmt, x, dt, rows, cols, ldx, codes, scales, (cudaStream_t)stream));
+    return ODY_OK;
+  });
+}
+
+extern "C" int ody_act8_load_on_stream(int32_t fmt, const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                                       int64_t cols, void* out, int32_t dt, int64_t ldo, void* stream) {
+  return guarded([&]() -> int {
+    if (int rc = act8_args(fmt, out, dt, rows, cols, ldo, codes, scales)) return rc;
+    if (int rc = act8_device(out, dt, codes, scales, "ody_act8_load_on_stream")) return rc;
+    ODY_CUDA(launch_act8_load(fmt, codes, scales, rows, cols, out, dt, ldo, (cudaStream_t)stream));
+    return ODY_OK;
+  });
+}
+
+extern "C" int ody_act8_save(int32_t fmt, const void* x, int32_t dt, int64_t rows, int64_t cols, uint8_t* codes,
+                             uint8_t* scales) {
+  return guarded([&]() -> int {
+    if (int rc = act8_args(fmt, x, dt, rows, cols, cols, codes, scales)) return rc;
+    const int64_t groups = ody_act8_groups(cols);
+    Scope S;
+    S.bufs.reserve(4);
+    void *dx, *dc, *ds;
+    ODY_STAGE(S, x, (size_t)(rows * cols) * dtype_size(dt), true, &dx);
+    ODY_STAGE(S, codes, (size_t)(rows * groups * kA8Group), false, &dc);
+    ODY_STAGE(S, scales, (size_t)(rows * groups), false, &ds);
+    if (int rc = act8_device(dx, dt, dc, ds, "ody_act8_save")) return rc;
+    ODY_CUDA(launch_act8_save(fmt, dx, dt, rows, cols, cols, (uint8_t*)dc, (uint8_t*)ds, S.st));
+    ODY_CUDA(S.copy_out(codes));
+    ODY_CUDA(S.copy_out(scales));
+    ODY_CUDA(cudaStreamSynchronize(S.st));
+    return ODY_OK;
+  });
+}
+
+extern "C" int ody_act8_load(int32_t fmt, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols,
+                             void* out, int32_t dt) {
+  return guarded([&]() -> int {
+    if (int rc = act8_args(fmt, out, dt, rows, cols, cols, codes, scales)) return rc;
+    const int64_t groups = ody_act8_groups(cols);
+    Scope S;
+    S.bufs.reserve(4);
+    void *dx, *dc, *ds;
+    ODY_STAGE(S, codes, (size_t)(rows * groups * kA8Group), true, &dc);
+    ODY_STAGE(S, scales, (size_t)(rows * groups), true, &ds);
+    ODY_STAGE(S, out, (size_t)(rows * cols) * dtype_size(dt), false, &dx);
+    if (int rc = act8_device(dx, dt, dc, ds, "ody_act8_load")) return rc;
+    ODY_CUDA(launch_act8_load(fmt, (const uint8_t*)dc, (const uint8_t*)ds, rows, cols, dx, dt, cols, S.st));
+    ODY_CUDA(S.copy_out(out));
+    ODY_CUDA(cudaStreamSynchronize(S.st));
+    return ODY_OK;
+  });
+}
+
+extern "C" int64_t ody_linear_workspace(int32_t op, int64_t rows, int64_t out, int64_t in, int32_t act_dtype) {
+  LinearArgs a{};
+  if (op < LIN_FORWARD || op > LIN_WGRAD || rows <= 0 || out <= 0 || in <= 0 || rows > kMaxDim || out > kMaxDim ||
+      in > kMaxDim || act_dtype < DT_F32 || act_dtype > DT_BF16)
+    return -1;
+  a.op = op;
+  a.rows = rows, a.out = out, a.in = in;
+  a.a_dtype = act_dtype;
+  return linear_workspace(a);
+}
+
+#define ODY_W4_PAIR(NAME, OP, ACT, OUT, ACOLS, CCOLS)                                                               \
+  extern "C" int NAME##_on_stream(int32_t kind, const void* q, const float* tensor_scale, float alpha,              \
+                                  int64_t out_features, int64_t in_features, const void* ACT, int32_t act_dtype,    \
+                                  int64_t rows, int64_t lda, void* OUT, int32_t out_dtype, int64_t ldo,             \
+                                  void* workspace, size_t workspace_bytes, void* stream) {                          \
+    return guarded([&]() -> int {                                                                                   \
+      LinearArgs a;                                                                                                 \
+      if (int rc = product(a, OP, kind, rows, out_features, in_features, ACT, act_dtype, lda, q, nullptr, OUT,      \
+                           out_dtype, ldo))                                                                         \
+        return rc;                                                                                                  \
+      a.o.alpha = alpha;                                                                                            \
+      a.o.tscale = tensor_scale;                                                                                    \
+      return on_stream(a, workspace, workspace_bytes, stream, #NAME "_on_stream");                                  \
+    });                                                                                                             \
+  }                                                                                                                 \
+  extern "C" int NAME(int32_t kind, const void* q, float tensor_scale, int64_t out_features, int64_t in_features,   \
+                      const void* ACT, int32_t act_dtype, int64_t rows, void* OUT, int32_t out_dtype) {             \
+    return guarded([&]() -> int {                                                                                   \
+      LinearArgs a;                                                                                                 \
+      if (int rc = product(a, OP, kind, rows, out_features, in_features, ACT, act_dtype, ACOLS, q, nullptr, OUT,    \
+                           out_dtype, CCOLS))                                                                       \
+        return rc;                                                                                                  \
+      return staged(a, kind == ODY_Q_NVFP4_TENSOR ? tensor_scale : 1.0f);                                           \
+    });                                                                                                             \
+  }
+
+ODY_W4_PAIR(ody_fp4_linear, LIN_FORWARD, x, y, in_features, out_features)
+ODY_W4_PAIR(ody_fp4_linear_dgrad, LIN_DGRAD, dy, dx, out_features, in_features)
+#undef ODY_W4_PAIR
+
+extern "C" int ody_linear_wgrad8_on_stream(int32_t fmt, const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                                           int64_t in_features, const void* dy, int32_t dy_dtype, int64_t out_features,
+                                           int64_t lddy, float alpha, const void* add, void* dw, int32_t dw_dtype,
+                                           void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&]() -> int {
+    LinearArgs a;
+    if (int rc = product(a, LIN_WGRAD, fmt, rows, out_features, in_features, dy, dy_dtype, lddy, codes, scales, dw,
+                         dw_dtype, in_features))
+      return rc;
+    a.o.alpha = alpha;
+    a.o.add = add;
+    if (reinterpret_cast<uintptr_t>(codes) & 15u)
+      return fail(ODY_ERR_ARG, "ody_linear_wgrad8_on_stream: codes must be 16-byte aligned");
+    return on_stream(a, workspace, workspace_bytes, stream, "ody_linear_wgrad8_on_stream");
+  });
+}
+
+extern "C" int ody_linear_wgrad8(int32_t fmt, const uint8_t* codes, const uint8_t* scales, int64_t rows,
+                                 int64_t in_features, const void* dy, int32_t dy_dtype, int64_t out_features,
+                                 float alpha, const void* add, void* dw, int32_t dw_dtype) {
+  return guarded([&]() -> int {
+    LinearArgs a;
+    if (int rc = product(a, LIN_WGRAD, fmt, rows, out_features, in_features, dy, dy_dtype, out_features, codes, scales,
+                         dw, dw_dtype, in_features))
+      return rc;
+    a.o.add = add;
+    if (is_device_ptr(codes) && (reinterpret_cast<uintptr_t>(codes) & 15u))
+      return fail(ODY_ERR_ARG, "ody_linear_wgrad8: codes must be 16-byte aligned");
+    return staged(a, alpha);
+  });
+}

@@ -1,0 +1,296 @@
+"""The linear layer over the update step's quantised weights, on
+libodyssey_mp.so (extensions; the reference's linear layer works on float
+tensors).
+
+    y  = fp4_linear(x, w)             y  = x W^T    W in 4 bits, as the step leaves it
+    dx = fp4_linear_dgrad(dy, w)      dx = dy W
+    a  = save_activation8(x)          x kept in 8 bits for the backward pass
+    x' = load_activation8(a)
+    dW = linear_wgrad8(dy, a)         dW = dy^T x'
+
+Weights are QuantizedTensors of the 4-bit kinds (to_mxfp4, to_nvfp4,
+to_nvfp4_tensor_scaled, to_mxfp4_ocp, MixedPrecisionStep.get_quant), read
+where they lie.  Activations and gradients are float32, float16 or bfloat16
+arrays whose last axis is the feature axis; leading axes are tokens.  CUDA
+tensors run on torch's current stream of their device without waiting, host
+arrays (numpy, or torch on the CPU; bfloat16 numpy data as uint16 with
+dtype='bfloat16') are staged and the call returns when done.
+"""
+import ctypes as C
+from dataclasses import dataclass
+
+import numpy as np
+
+from . import _lib as L
+from .quant import QuantizedTensor
+
+FORMATS8 = {"e4m3": L.A8_E4M3, "e5m2": L.A8_E5M2}
+_NAMES = ("float32", "float16", "bfloat16")
+_CODES = {"float32": L.F32, "float16": L.F16, "bfloat16": L.BF16, L.F32: L.F32, L.F16: L.F16, L.BF16: L.BF16}
+_W4 = (L.Q_MXFP4, L.Q_NVFP4, L.Q_NVFP4_TENSOR, L.Q_MXFP4_OCP)
+_TORCH = {}
+
+
+def _torch_dtypes():
+    t = L._torch()
+    if not _TORCH and t is not None:
+        _TORCH.update({t.float32: L.F32, t.float16: L.F16, t.bfloat16: L.BF16,
+                       L.F32: t.float32, L.F16: t.float16, L.BF16: t.bfloat16})
+    return _TORCH
+
+
+def _code(dtype):
+    """F32/F16/BF16 code of a dtype given by name, code or torch dtype."""
+    c = _CODES.get(dtype) if isinstance(dtype, (str, int)) else _torch_dtypes().get(dtype)
+    if c is None:
+        raise L.OdysseyError(f"unsupported dtype {dtype}", L.ERR_DTYPE)
+    return c
+
+
+@dataclass
+class Activation8:
+    """An activation in 8 bits: codes [rows, 32 * groups] and one scale byte
+    per row and 32 columns, uint8; `shape` and `dtype` are the saved tensor's
+    (None: [rows, cols] and bfloat16)."""
+    codes: object
+    scales: object
+    rows: int
+    cols: int
+    format: str = "e4m3"
+    shape: tuple = None
+    dtype: object = None
+
+    def check(self):
+        g = (self.cols + 31) // 32
+        if self.format not in FORMATS8:
+            raise L.OdysseyError(f"unknown 8-bit activation format {self.format!r}", L.ERR_ARG)
+        if self.rows <= 0 or self.cols <= 0:
+            raise L.OdysseyError("cannot save an empty activation", L.ERR_SHAPE)
+        if L.numel(self.codes) != self.rows * g * 32 or L.numel(self.scales) != self.rows * g:
+            raise L.OdysseyError("codes and scales do not have the bytes of the activation's rows and columns",
+                                 L.ERR_SHAPE)
+        for b in (self.codes, self.scales):
+            if (b.dtype.itemsize if L.is_torch(b) else np.asarray(b).itemsize) != 1:
+                raise L.OdysseyError("codes and scales must be uint8", L.ERR_DTYPE)
+
+
+class _Rows:
+    """An array as rows of its last axis: the code of its type, pitch, and
+    (for CUDA tensors) the device and torch's current stream on it."""
+    __slots__ = ("a", "code", "rows", "cols", "ld", "cuda", "ptr", "lead")
+
+    def __init__(self, x, dtype, what):
+        if L.is_torch(x):
+            code = _torch_dtypes().get(x.dtype)
+            if code is None:
+                raise L.OdysseyError(f"unsupported dtype {x.dtype}", L.ERR_DTYPE)
+            shape = x.shape
+            if len(shape) == 0 or x.numel() == 0:
+                raise L.OdysseyError(f"{what} is empty", L.ERR_SHAPE)
+            self.cuda = x.is_cuda
+            if x.dim() != 2:
+                x = x.reshape(-1, shape[-1])
+            # rows of any pitch are read in place; anything else is copied
+            if x.stride(1) != 1 and x.shape[1] > 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1] or not self.cuda:
+                x = x.contiguous()
+            self.ld = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+            self.ptr = x.data_ptr()
+        else:
+            code = L.dtype_code(x, dtype)
+            shape = np.shape(x)
+            x = np.ascontiguousarray(x)
+            if len(shape) == 0 or x.size == 0:
+                raise L.OdysseyError(f"{what} is empty", L.ERR_SHAPE)
+            self.cuda = False
+            x = x.reshape(-1, shape[-1])
+            self.ld = x.shape[1]
+            self.ptr = x.ctypes.data
+        self.a, self.code, self.lead = x, code, tuple(shape[:-1])
+        self.rows, self.cols = x.shape
+
+
+def _same_place(x, *others):
+    """Buffers of one call live on one device (or all on the host)."""
+    for o in others:
+        if o is None:
+            continue
+        t = L.is_torch(o) and o.is_cuda
+        if t != x.cuda or (t and o.device != x.a.device):
+            raise L.OdysseyError("the buffers of a call must be on one device", L.ERR_ARG)
+
+
+def _out(x, out, shape, code, what):
+    """The result buffer: new, or the caller's after its checks."""
+    if out is None:
+        if L.is_torch(x.a):
+            return L._torch().empty(shape, dtype=_torch_dtypes()[code], device=x.a.device)
+        return np.empty(shape, (np.float32, np.float16, np.uint16)[code])
+    _same_place(x, out)
+    have = _torch_dtypes().get(out.dtype) if L.is_torch(out) else \
+        {np.dtype(np.float32): L.F32, np.dtype(np.float16): L.F16, np.dtype(np.uint16): L.BF16}.get(out.dtype)
+    if have != code:
+        raise L.OdysseyError(f"{what} must be {_NAMES[code]}", L.ERR_DTYPE)
+    if tuple(out.shape) != tuple(shape):
+        raise L.OdysseyError(f"{what} has shape {tuple(out.shape)}, expected {tuple(shape)}", L.ERR_SHAPE)
+    L.ptr(out)  # contiguous
+    return out
+
+
+class _On:
+    """The device of a CUDA call made current, and torch's stream on it."""
+
+    def __init__(self, device):
+        t = L._torch()
+        self.guard = t.cuda.device(device) if device.index != t.cuda.current_device() else None
+        self.device = device
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return L._torch().cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+def _workspace(op, rows, out, inn, code, device):
+    n = L.lib().ody_linear_workspace(op, rows, out, inn, code)
+    if n <= 0:
+        return None, 0, 0
+    ws = L._torch().empty(n, dtype=L._torch().uint8, device=device)
+    return ws, ws.data_ptr(), n
+
+
+def _product(name, op, x, w, out, out_dtype, dtype, what):
+    if not isinstance(w, QuantizedTensor) or w.kind not in _W4:
+        raise L.OdysseyError(f"{name} takes a weight of the 4-bit kinds", L.ERR_ARG)
+    r = _Rows(x, dtype, what)
+    features, numel = r.cols, w.original_numel
+    other = numel // features
+    if numel <= 0 or other * features != numel:
+        raise L.OdysseyError(f"{name}: a weight of {numel} elements has no rows of {features}" if op == L.LINEAR_FORWARD
+                             else f"{name}: a weight of {numel} elements does not have {features} rows", L.ERR_SHAPE)
+    nout, nin = (other, features) if op == L.LINEAR_FORWARD else (features, other)
+    if L.numel(w.data) != L.quant_bytes(w.kind, numel):
+        raise L.OdysseyError(f"quantised buffer has {L.numel(w.data)} bytes, expected "
+                             f"{L.quant_bytes(w.kind, numel)}", L.ERR_SHAPE)
+    code = r.code if out_dtype is None else _code(out_dtype)
+    y = _out(r, out, r.lead + (other,), code, "out")
+    lib = L.lib()
+    if r.cuda:
+        _same_place(r, w.data)
+        data = w.data if w.data.is_contiguous() else w.data.contiguous()
+        ts, alpha = None, 1.0
+        if w.kind == L.Q_NVFP4_TENSOR:
+            if L.is_torch(w.tensor_scale):  # a device float: read by the kernel, no synchronisation
+                _same_place(r, w.tensor_scale)
+                if w.tensor_scale.numel() != 1 or w.tensor_scale.dtype != L._torch().float32:
+                    raise L.OdysseyError("the tensor scale must be one float32", L.ERR_DTYPE)
+                ts = w.tensor_scale.data_ptr()
+            else:
+                alpha = w.tensor_scale
+        fn = lib.ody_fp4_linear_on_stream if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad_on_stream
+        with _On(r.a.device) as st:
+            ws, wp, wn = _workspace(op, r.rows, nout, nin, r.code, r.a.device)
+            L.check(fn(w.kind, data.data_ptr(), ts, alpha, nout, nin, r.ptr, r.code, r.rows, r.ld, y.data_ptr(), code,
+                       other, wp, wn, st))
+        return y
+    _same_place(r, w.data)
+    fn = lib.ody_fp4_linear if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad
+    L.check(fn(w.kind, L.ptr(L.contiguous(w.data)), float(w.tensor_scale), nout, nin, r.ptr, r.code, r.rows, L.ptr(y),
+               code))
+    return y
+
+
+def fp4_linear(x, w, out=None, out_dtype=None, dtype=None):
+    """y[..., out_features] = x[..., in_features] W^T with W the 4-bit weight
+    [w.original_numel / in_features, in_features].  out_dtype: x's by default."""
+    return _product("fp4_linear", L.LINEAR_FORWARD, x, w, out, out_dtype, dtype, "x")
+
+
+def fp4_linear_dgrad(dy, w, out=None, out_dtype=None, dtype=None):
+    """dx[..., in_features] = dy[..., out_features] W, the input gradient of
+    fp4_linear.  out_dtype: dy's by default."""
+    return _product("fp4_linear_dgrad", L.LINEAR_DGRAD, dy, w, out, out_dtype, dtype, "dy")
+
+
+def save_activation8(x, format="e4m3", dtype=None):
+    """x[..., cols] in 8 bits ('e4m3' or 'e5m2') with a power of two per 32
+    columns, the least that keeps the group's largest finite element in range."""
+    if format not in FORMATS8:
+        raise L.OdysseyError(f"unknown 8-bit activation format {format!r}", L.ERR_ARG)
+    r = _Rows(x, dtype, "x")
+    g = (r.cols + 31) // 32
+    if L.is_torch(r.a):
+        t = L._torch()
+        # one allocation: the codes' rows, then the scales
+        buf = t.empty(r.rows * g * 33, dtype=t.uint8, device=r.a.device)
+        codes, scales = buf[:r.rows * g * 32].view(r.rows, g * 32), buf[r.rows * g * 32:].view(r.rows, g)
+    else:
+        codes, scales = np.empty((r.rows, g * 32), np.uint8), np.empty((r.rows, g), np.uint8)
+    if r.cuda:
+        with _On(r.a.device) as st:
+            L.check(L.lib().ody_act8_save_on_stream(FORMATS8[format], r.ptr, r.code, r.rows, r.cols, r.ld,
+                                                    codes.data_ptr(), scales.data_ptr(), st))
+    else:
+        L.check(L.lib().ody_act8_save(FORMATS8[format], r.ptr, r.code, r.rows, r.cols, L.ptr(codes), L.ptr(scales)))
+    return Activation8(codes, scales, r.rows, r.cols, format, r.lead + (r.cols,), _NAMES[r.code])
+
+
+def load_activation8(a, dtype=None, out=None):
+    """The values an Activation8 stands for, in the saved shape and type (or `dtype`)."""
+    a.check()
+    code = _code(dtype if dtype is not None else a.dtype if a.dtype is not None else L.BF16)
+    shape = a.shape if a.shape is not None else (a.rows, a.cols)
+    codes, scales = L.contiguous(a.codes), L.contiguous(a.scales)
+    r = _Place(codes)
+    _same_place(r, scales)
+    y = _out(r, out, shape, code, "out")
+    fn, c, s = L.lib(), L.ptr(codes), L.ptr(scales)
+    if r.cuda:
+        with _On(codes.device) as st:
+            L.check(fn.ody_act8_load_on_stream(FORMATS8[a.format], c, s, a.rows, a.cols, y.data_ptr(), code, a.cols, st))
+    else:
+        L.check(fn.ody_act8_load(FORMATS8[a.format], c, s, a.rows, a.cols, L.ptr(y), code))
+    return y
+
+
+class _Place:
+    """Where a buffer lies (what _same_place and _out ask of _Rows)."""
+
+    def __init__(self, a):
+        self.a, self.cuda = a, L.is_torch(a) and a.is_cuda
+
+
+def linear_wgrad8(dy, a, add=None, alpha=1.0, out=None, out_dtype=None, dtype=None):
+    """dW[out_features, in_features] = alpha dy^T x' (+ add) from dy[...,
+    out_features] and the activation saved in the forward pass.  add: of the
+    result's type; it may be `out` (accumulation in place).  out_dtype: add's,
+    out's or dy's."""
+    a.check()
+    r = _Rows(dy, dtype, "dy")
+    if r.rows != a.rows:
+        raise L.OdysseyError(f"dy has {r.rows} rows, the saved activation {a.rows}", L.ERR_SHAPE)
+    _same_place(r, a.codes, a.scales)
+    if out_dtype is not None:
+        code = _code(out_dtype)
+    else:
+        like = out if out is not None else add
+        code = r.code if like is None else \
+            (L.BF16 if not L.is_torch(like) and like.dtype == np.uint16 else L.dtype_code(like))
+    y = _out(r, out, (r.cols, a.cols), code, "out")
+    if add is not None:
+        add = _out(r, add, (r.cols, a.cols), code, "add")
+    codes, scales = L.contiguous(a.codes), L.contiguous(a.scales)
+    fmt, lib = FORMATS8[a.format], L.lib()
+    if r.cuda:
+        with _On(r.a.device) as st:
+            ws, wp, wn = _workspace(L.LINEAR_WGRAD, r.rows, r.cols, a.cols, r.code, r.a.device)
+            L.check(lib.ody_linear_wgrad8_on_stream(fmt, codes.data_ptr(), scales.data_ptr(), a.rows, a.cols, r.ptr,
+                                                    r.code, r.cols, r.ld, alpha, None if add is None else add.data_ptr(),
+                                                    y.data_ptr(), code, wp, wn, st))
+    else:
+        L.check(lib.ody_linear_wgrad8(fmt, L.ptr(codes), L.ptr(scales), a.rows, a.cols, r.ptr, r.code, r.cols,
+                                      C.c_float(alpha), None if add is None else L.ptr(add), L.ptr(y), code))
+    return y
