@@ -423,6 +423,11 @@ int ody_dequant_bf16(const void* q, int64_t n, float* out);   /* the exact BF16 
 #define ODY_LINEAR_WGRAD 2
 /* workspace bytes of one call (-1: bad arguments); act_dtype is x's or dy's */
 int64_t ody_linear_workspace(int32_t op, int64_t rows, int64_t out_features, int64_t in_features, int32_t act_dtype);
+/* Waits for `stream` and reports what the calls on the current GPU cannot
+ * return: ODY_ERR_DEVICE_BOUNDS if a wait inside one of their kernels ran out
+ * (each is bounded by 2 s; results of that call are then incomplete) since
+ * the last query, else ODY_OK.  The plain forms query it themselves. */
+int ody_linear_status(void* stream);
 int ody_fp4_linear_on_stream(int32_t kind, const void* q, const float* tensor_scale, float alpha,
                              int64_t out_features, int64_t in_features, const void* x, int32_t x_dtype, int64_t rows,
                              int64_t ldx, void* y, int32_t y_dtype, int64_t ldy, void* workspace,

@@ -14,8 +14,8 @@ from ._lib import LIB_PATH, OdysseyError, lib  # noqa: F401
 from .fused import MixedPrecisionStep, nccl_unique_id, plan_shards  # noqa: F401
 from .gradient_clipping import (clip_global_norm, clip_grad_global_norm_,  # noqa: F401
                                 clip_gradients_by_global_norm, compute_gradient_norm_list)
-from .linear import (Activation8, fp4_linear, fp4_linear_dgrad, linear_wgrad8, load_activation8,  # noqa: F401
-                     save_activation8)
+from .linear import (Activation8, fp4_linear, fp4_linear_dgrad, linear_status, linear_wgrad8,  # noqa: F401
+                     load_activation8, save_activation8)
 from .mixed_precision import (GradientScaler, check_gradients_finite, clip_gradients_by_norm,  # noqa: F401
                               convert_to_fp32_master, update_model_from_master)
 from .optimizers import (adagrad_step, adagrad_step_simple, adam_step, adamw_step,  # noqa: F401

@@ -15,8 +15,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libodyssey_mp.so")
-SOURCES = ["ody_kernels.cu", "ody_capi.cu", "ody_noalloc.cu", "ody_linear.cu", "ody_linear_capi.cu"]
-HEADERS = ["ody_internal.h", "ody_numerics.cuh", "ody_fp4fast.cuh", "ody_host.h", "ody_linear.h"]
+SOURCES = ["ody_kernels.cu", "ody_capi.cu", "ody_noalloc.cu", "ody_linear.cu", "ody_linear_gemm.cu",
+           "ody_linear_capi.cu"]
+HEADERS = ["ody_internal.h", "ody_numerics.cuh", "ody_fp4fast.cuh", "ody_host.h", "ody_linear.h",
+           "ody_linear_dev.cuh", "ody_linear_gemm.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ARCH + [
@@ -47,15 +49,18 @@ def build(force=False, verbose=False):
         return LIB
     objdir = os.path.join(HERE, "_build")
     os.makedirs(objdir, exist_ok=True)
-    objs = []
-    for src in SOURCES:
+    objs, running = [], []
+    for src in SOURCES:  # one nvcc each, side by side
         obj = os.path.join(objdir, src.replace(".cu", ".o"))
         cmd = [nvcc()] + NVFLAGS + ["-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
             print(" ".join(cmd))
-        subprocess.run(cmd, check=True)
+        running.append((cmd, subprocess.Popen(cmd)))
         objs.append(obj)
+    failed = [(cmd, rc) for cmd, rc in [(cmd, p.wait()) for cmd, p in running] if rc]
+    if failed:
+        raise subprocess.CalledProcessError(failed[0][1], failed[0][0])
     tmp = LIB + ".tmp"
     subprocess.run([nvcc()] + ARCH + ["-shared", "-o", tmp] + objs + ["-ldl"], check=True)
     os.replace(tmp, LIB)

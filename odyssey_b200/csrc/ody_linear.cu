@@ -10,74 +10,10 @@
 // elements, 9 for 16), so a block may straddle two rows.  x' are 8-bit codes
 // in rows of whole 32-column groups with one power of two per group.
 #include "ody_linear.h"
-
-#include "ody_numerics.cuh"
+#include "ody_linear_dev.cuh"
+#include "ody_linear_gemm.h"
 
 namespace ody {
-
-// ---------------------------------------------------------------------------
-// Decoding
-// ---------------------------------------------------------------------------
-template <int KIND>
-struct W4 {
-  static constexpr bool MX = KIND == Q_MXFP4 || KIND == Q_MXFP4_OCP;
-  static constexpr int BE = MX ? 32 : 16;  // elements per block
-  static constexpr int SB = MX ? 17 : 9;   // bytes per block
-
-  // a block's scale: E8M0 (in the OCP kind 0 is 2^-127 and 255 NaN) or E4M3
-  static __device__ __forceinline__ float scale(uint32_t b) {
-    if (KIND == Q_MXFP4_OCP)
-      return b == 0xFF ? __uint_as_float(0x7fc00000u) : (b ? __uint_as_float(b << 23) : __uint_as_float(0x00400000u));
-    if (KIND == Q_MXFP4) return e8m0_to_f32((uint8_t)b);
-    return e4m3_to_f32((uint8_t)b);
-  }
-  // code times scale; exact in float32 and, for finite scales, in bfloat16:
-  // two bits of value times at most four of scale.  Code 1 is 0.5 in the OCP
-  // kind and 0 in the others, and their zero is not multiplied by the scale.
-  static __device__ __forceinline__ float value(uint32_t code, float sf) {
-    if (KIND == Q_MXFP4_OCP) {
-      const uint32_t e = (code >> 1) & 3u, m = code & 1u;
-      const float un = e ? (m ? 1.5f : 1.0f) * (float)(1u << (e - 1)) : 0.5f * (float)m;
-      const float r = __fmul_rn(un, sf);
-      return code & 8u ? -r : r;
-    }
-    return fp4_decode(code, sf);
-  }
-  static __device__ __forceinline__ float at(const uint8_t* q, int64_t e) {
-    const uint8_t* blk = q + (e / BE) * SB;
-    const int i = (int)(e % BE);
-    const uint32_t b = blk[i >> 1];
-    return value(i & 1 ? b & 15u : b >> 4, scale(blk[SB - 1]));
-  }
-};
-
-template <int FMT>
-__device__ __forceinline__ float a8_value(uint32_t code, uint32_t scale_byte) {
-  const float v = FMT == A8_E4M3 ? e4m3_to_f32((uint8_t)code) : e5m2_to_f32((uint8_t)code);
-  return __fmul_rn(v, __uint_as_float(scale_byte << 23));
-}
-
-__device__ __forceinline__ float load_elem(const void* p, int dt, int64_t i) {
-  if (dt == DT_F32) return reinterpret_cast<const float*>(p)[i];
-  const uint16_t h = reinterpret_cast<const uint16_t*>(p)[i];
-  return dt == DT_F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h);
-}
-__device__ __forceinline__ void store_elem(void* p, int dt, int64_t i, float v) {
-  if (dt == DT_F32)
-    reinterpret_cast<float*>(p)[i] = v;
-  else
-    reinterpret_cast<uint16_t*>(p)[i] = dt == DT_F16 ? f32_to_f16_bits(v) : f32_to_bf16_bits(v);
-}
-
-__device__ __forceinline__ float out_scale(const LinearOut& o) {
-  return o.tscale ? __fmul_rn(o.alpha, *o.tscale) : o.alpha;
-}
-__device__ __forceinline__ void finish(const LinearOut& o, float s, int64_t i, int64_t j, float acc) {
-  const int64_t at = i * o.ld + j;
-  float v = __fmul_rn(acc, s);
-  if (o.add) v = __fadd_rn(v, load_elem(o.add, o.dtype, at));
-  store_elem(o.c, o.dtype, at, v);
-}
 
 // ---------------------------------------------------------------------------
 // Products on the FP32 pipe: 64 x 64 tiles, 256 threads with 4 x 4 results
@@ -167,14 +103,23 @@ static cudaError_t launch_fp32_w4(const LinearArgs& a, cudaStream_t st) {
   }
 }
 
-int64_t linear_workspace(const LinearArgs& a) {
-  (void)a;
-  return 0;
+static int lin_sms() {
+  static int n[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return 148;
+  if (!n[dev]) cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev);
+  return n[dev] ? n[dev] : 148;
 }
 
-cudaError_t launch_linear(const LinearArgs& a, void* ws, size_t ws_bytes, cudaStream_t st) {
-  (void)ws;
-  (void)ws_bytes;
+// Few products are done by the FP32 pipe in one launch; more go to the tensor
+// cores, after their operands have been brought to bfloat16.
+static bool small_product(const LinearArgs& a) { return (double)a.rows * a.out * a.in <= 0; }
+
+int64_t linear_workspace(const LinearArgs& a) { return small_product(a) ? 0 : gemm_workspace(a, lin_sms()); }
+
+cudaError_t launch_linear(const LinearArgs& a, void* ws, cudaStream_t st) {
+  if (!small_product(a)) return launch_gemm(a, ws, lin_sms(), st);
   if (a.op == LIN_FORWARD) return launch_fp32_w4<LIN_FORWARD>(a, st);
   if (a.op == LIN_DGRAD) return launch_fp32_w4<LIN_DGRAD>(a, st);
   return a.kind == A8_E4M3 ? launch_fp32<LIN_WGRAD, A8_E4M3>(a, st) : launch_fp32<LIN_WGRAD, A8_E5M2>(a, st);
@@ -310,15 +255,6 @@ __global__ void __launch_bounds__(256) act8_load_kernel(const uint8_t* codes, co
         if (c0 + i < cols) store_elem(out, DT, at + i, v[i]);
     }
   }
-}
-
-static int lin_sms() {
-  static int n[64] = {0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return 148;
-  if (!n[dev]) cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev);
-  return n[dev] ? n[dev] : 148;
 }
 
 static int act8_grid(int64_t rows, int64_t cols) {

@@ -39,7 +39,7 @@ constexpr int kA8Group = 32;
 // bytes of workspace launch_linear may use for these shapes and types,
 // whatever the pointers' alignment and the strides
 int64_t linear_workspace(const LinearArgs& a);
-cudaError_t launch_linear(const LinearArgs& a, void* ws, size_t ws_bytes, cudaStream_t st);
+cudaError_t launch_linear(const LinearArgs& a, void* ws, cudaStream_t st);
 cudaError_t launch_act8_save(int fmt, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes,
                              uint8_t* scales, cudaStream_t st);
 cudaError_t launch_act8_load(int fmt, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* out,

@@ -5,6 +5,7 @@
 
 #include "ody_host.h"
 #include "ody_linear.h"
+#include "ody_linear_gemm.h"
 
 using namespace ody;
 
@@ -67,11 +68,11 @@ int aligned_to(const void* p, int dtype, const char* what) {
   return ODY_OK;
 }
 
-int launch(const LinearArgs& a, void* ws, size_t ws_bytes, cudaStream_t st) {
+int launch(const LinearArgs& a, void* ws, cudaStream_t st) {
   if (aligned_to(a.a, a.a_dtype, "an operand") || aligned_to(a.o.c, a.o.dtype, "the output") ||
       (a.o.add && aligned_to(a.o.add, a.o.dtype, "add")))
     return ODY_ERR_ARG;
-  ODY_CUDA(launch_linear(a, ws, ws_bytes, st));
+  ODY_CUDA(launch_linear(a, ws, st));
   return ODY_OK;
 }
 
@@ -85,7 +86,14 @@ int on_stream(const LinearArgs& a, void* ws, size_t ws_bytes, void* stream, cons
     return fail(ODY_ERR_ARG, std::string(name) + " takes memory of the current GPU only");
   if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 255u))
     return fail(ODY_ERR_ARG, std::string(name) + ": the workspace must be 256-byte aligned");
-  return launch(a, ws, ws_bytes, (cudaStream_t)stream);
+  return launch(a, ws, (cudaStream_t)stream);
+}
+
+// waits for the stream; whether a bounded wait on the device ran out
+int status(cudaStream_t st) {
+  bool ran_out = false;
+  ODY_CUDA(gemm_wait_error(st, &ran_out));
+  return ran_out ? fail(ODY_ERR_DEVICE_BOUNDS, "a bounded wait inside a linear kernel ran out") : ODY_OK;
 }
 
 // host or device buffers, contiguous; waits for the result
@@ -112,10 +120,9 @@ int staged(LinearArgs a, float alpha) {
     S.bufs.push_back({nullptr, ws, 0, true});
   }
   a.a = da, a.q = (const uint8_t*)dq, a.scales = (const uint8_t*)ds, a.o.c = dc, a.o.add = dadd;
-  if (int rc = launch(a, ws, (size_t)need, S.st)) return rc;
+  if (int rc = launch(a, ws, S.st)) return rc;
   ODY_CUDA(S.copy_out(c));
-  ODY_CUDA(cudaStreamSynchronize(S.st));
-  return ODY_OK;
+  return status(S.st);
 }
 
 int act8_args(int32_t fmt, const void* x, int32_t dt, int64_t rows, int64_t cols, int64_t ld, const void* codes,
@@ -272,4 +279,15 @@ extern "C" int ody_linear_wgrad8(int32_t fmt, const uint8_t* codes, const uint8_
       return fail(ODY_ERR_ARG, "ody_linear_wgrad8: codes must be 16-byte aligned");
     return staged(a, alpha);
   });
+}
+
+extern "C" int ody_linear_status(void* stream) {
+  return guarded([&]() -> int { return status((cudaStream_t)stream); });
+}
+
+// Test hook (not part of include/odyssey_mp.h): a device-side wait that runs
+// out after limit_ns.
+extern "C" int odyx_linear_wait_selftest(uint64_t limit_ns, void* stream) {
+  ODY_CUDA(launch_wait_selftest(limit_ns, (cudaStream_t)stream));
+  return ODY_OK;
 }

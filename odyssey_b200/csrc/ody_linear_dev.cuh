@@ -1,0 +1,91 @@
+// ody_linear_dev.cuh -- device pieces shared by the quantised linear layer's
+// kernels: decoding of 4-bit weights and 8-bit activations, element access,
+// the last step of a result.
+#pragma once
+#include "ody_linear.h"
+#include "ody_numerics.cuh"
+
+namespace ody {
+
+template <int KIND>
+struct W4 {
+  static constexpr bool MX = KIND == Q_MXFP4 || KIND == Q_MXFP4_OCP;
+  static constexpr int BE = MX ? 32 : 16;  // elements per block
+  static constexpr int SB = MX ? 17 : 9;   // bytes per block
+
+  // a block's scale: E8M0 (in the OCP kind 0 is 2^-127 and 255 NaN) or E4M3
+  static __device__ __forceinline__ float scale(uint32_t b) {
+    if (KIND == Q_MXFP4_OCP)
+      return b == 0xFF ? __uint_as_float(0x7fc00000u) : (b ? __uint_as_float(b << 23) : __uint_as_float(0x00400000u));
+    if (KIND == Q_MXFP4) return e8m0_to_f32((uint8_t)b);
+    return e4m3_to_f32((uint8_t)b);
+  }
+  // code times scale; exact in float32 and, for finite scales, in bfloat16:
+  // two bits of value times at most four of scale.  Code 1 is 0.5 in the OCP
+  // kind and 0 in the others, and their zero is not multiplied by the scale.
+  static __device__ __forceinline__ float value(uint32_t code, float sf) {
+    if (KIND == Q_MXFP4_OCP) {
+      const uint32_t e = (code >> 1) & 3u, m = code & 1u;
+      const float un = e ? (m ? 1.5f : 1.0f) * (float)(1u << (e - 1)) : 0.5f * (float)m;
+      const float r = __fmul_rn(un, sf);
+      return code & 8u ? -r : r;
+    }
+    return fp4_decode(code, sf);
+  }
+  static __device__ __forceinline__ float at(const uint8_t* q, int64_t e) {
+    const uint8_t* blk = q + (e / BE) * SB;
+    const int i = (int)(e % BE);
+    const uint32_t b = blk[i >> 1];
+    return value(i & 1 ? b & 15u : b >> 4, scale(blk[SB - 1]));
+  }
+};
+
+template <int FMT>
+__device__ __forceinline__ float a8_value(uint32_t code, uint32_t scale_byte) {
+  const float v = FMT == A8_E4M3 ? e4m3_to_f32((uint8_t)code) : e5m2_to_f32((uint8_t)code);
+  return __fmul_rn(v, __uint_as_float(scale_byte << 23));
+}
+
+__device__ __forceinline__ float load_elem(const void* p, int dt, int64_t i) {
+  if (dt == DT_F32) return reinterpret_cast<const float*>(p)[i];
+  const uint16_t h = reinterpret_cast<const uint16_t*>(p)[i];
+  return dt == DT_F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h);
+}
+__device__ __forceinline__ void store_elem(void* p, int dt, int64_t i, float v) {
+  if (dt == DT_F32)
+    reinterpret_cast<float*>(p)[i] = v;
+  else
+    reinterpret_cast<uint16_t*>(p)[i] = dt == DT_F16 ? f32_to_f16_bits(v) : f32_to_bf16_bits(v);
+}
+
+__device__ __forceinline__ float out_scale(const LinearOut& o) {
+  return o.tscale ? __fmul_rn(o.alpha, *o.tscale) : o.alpha;
+}
+__device__ __forceinline__ void finish(const LinearOut& o, float s, int64_t i, int64_t j, float acc) {
+  const int64_t at = i * o.ld + j;
+  float v = __fmul_rn(acc, s);
+  if (o.add) v = __fadd_rn(v, load_elem(o.add, o.dtype, at));
+  store_elem(o.c, o.dtype, at, v);
+}
+
+// A float32 as the exact sum of three bfloat16 (float16: of two): each part
+// is the rest cut to bfloat16's eight bits, so no part is ever larger than
+// the value (rounding up could pass the largest finite one).  A non-finite
+// value is its first part alone, since inf - inf would spoil the others.
+__device__ __forceinline__ void split_bf16(float x, uint16_t& a, uint16_t& b, uint16_t& c) {
+  const uint32_t u = __float_as_uint(x);
+  if ((u & 0x7f800000u) == 0x7f800000u) {
+    a = (u & 0x7fffffu) ? 0x7fc0 : (uint16_t)(u >> 16);
+    b = c = 0;
+    return;
+  }
+  a = (uint16_t)(u >> 16);
+  const float r = __fsub_rn(x, __uint_as_float(u & 0xffff0000u));
+  const uint32_t v = __float_as_uint(r);
+  b = (uint16_t)(v >> 16);
+  c = (uint16_t)(__float_as_uint(__fsub_rn(r, __uint_as_float(v & 0xffff0000u))) >> 16);
+}
+// parts an element of this type takes
+__host__ __device__ constexpr int bf16_parts(int dtype) { return dtype == DT_F32 ? 3 : (dtype == DT_F16 ? 2 : 1); }
+
+}  // namespace ody

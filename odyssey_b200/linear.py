@@ -294,3 +294,12 @@ def linear_wgrad8(dy, a, add=None, alpha=1.0, out=None, out_dtype=None, dtype=No
         L.check(lib.ody_linear_wgrad8(fmt, L.ptr(codes), L.ptr(scales), a.rows, a.cols, r.ptr, r.code, r.cols,
                                       C.c_float(alpha), None if add is None else L.ptr(add), L.ptr(y), code))
     return y
+
+
+def linear_status(device=None):
+    """Waits for torch's current stream of the device and raises if a bounded
+    wait inside a linear kernel ran out there since the last query (the CUDA
+    calls above do not wait, so they cannot say so themselves)."""
+    t = L._torch()
+    with _On(t.device("cuda", t.cuda.current_device() if device is None else t.device(device).index)) as st:
+        L.check(L.lib().ody_linear_status(st))
