@@ -139,21 +139,29 @@ __global__ void __launch_bounds__(256) pack_planes_kernel(const void* __restrict
 // ---------------------------------------------------------------------------
 // The product: C[m, n] = sum over planes and r of A_p(m, r) B(n, r)
 //
-// Persistent CTAs, one per SM.  Warp 0 copies 128 x 64 of A and 256 x 64 of B
-// per step by TMA (128-byte swizzle) through four stages; warp 1 issues four
-// tcgen05.mma (128 x 256 x 16) per step into one of two TMEM accumulators;
-// warps 4 to 11 take a finished accumulator out.  An operand whose rows are
-// the reduction's (dgrad's W, both of wgrad's) is copied the same way, 64
-// columns at a time, and multiplied as "MN-major".
+// Persistent CTA pairs, one CTA per SM, 256 x 256 results per pair.  In each
+// CTA warp 0 copies its 128 x 64 of A and its 128 x 64 of B per step by TMA
+// (128-byte swizzle) through six stages; the first CTA's warp 1 issues four
+// tcgen05.mma.cta_group::2 (256 x 256 x 16) per step, which read both CTAs'
+// halves, into one of two TMEM accumulators; warps 4 to 11 of each CTA take
+// its 128 finished rows out.  The pair halves what every SM loads: one CTA
+// alone with 128 x 256 results needs 48 KB per 512 cycles of MMA from L2 and
+// reached 0.54 of the pair's rate.
+//
+// An operand whose rows are the reduction's (dgrad's W, both of wgrad's) is
+// copied the same way, 64 columns at a time, and multiplied as "MN-major".
 //
 // The tensor core cuts off the low bits of what it adds, so a long sum in one
-// accumulator drifts; every kChunk steps the accumulator is therefore taken
+// accumulator drifts; every 256 products the accumulator is therefore taken
 // to registers and added there in float32 with rounding, while the tensor
 // core fills the other one.
 // ---------------------------------------------------------------------------
-constexpr int kBM = 128, kBN = 256, kBK = 64, kStages = 4, kChunk64 = 4;
-constexpr int kABytes = kBM * kBK * 2, kBBytes = kBN * kBK * 2, kStageBytes = kABytes + kBBytes;
-constexpr int kGemmSmem = kStages * kStageBytes + 1024;
+constexpr int kBM = 256, kBN = 256, kBK = 64, kStages = 6, kChunk64 = 4;
+constexpr int kHalf = 128;                                   // rows of A and of B in each CTA
+constexpr int kHalfBytes = kHalf * kBK * 2, kStageBytes = 2 * kHalfBytes;
+constexpr int kStagePitch = 33;                              // floats; the epilogue's 32 x 32 transposes
+constexpr int kEpiBytes = 8 * 32 * kStagePitch * 4;
+constexpr int kGemmSmem = kStages * kStageBytes + kEpiBytes + 1024;
 constexpr int kGemmThreads = 384;
 constexpr unsigned long long kGemmWaitNs = 2000000000ull;  // bound on every wait (2 s)
 
@@ -169,7 +177,8 @@ __device__ __forceinline__ unsigned long long now_ns() {
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
       : "memory");
@@ -193,28 +202,41 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {  // the same place in a CTA of the pair
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// a box into this CTA's memory; its bytes count on a barrier of either CTA
 __device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          dst),
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
+// arrives at the barrier in both CTAs when the MMAs issued so far are done
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                   bar),
+               "h"((uint16_t)3)
+               : "memory");
 }
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Shared-memory descriptor of a 128-byte-swizzled operand: K-major, rows of
 // 64 k at 128 bytes, eight rows every 1024 bytes; MN-major, the same rows are
@@ -243,9 +265,42 @@ __device__ __forceinline__ void tile_at(const GemmArgs& g, int t, int& tm, int& 
   tm = first + in % h;
   tn = in / h;
 }
+__device__ __forceinline__ int split_at(const GemmArgs& g, int sp) {
+  return (int)((int64_t)g.steps * g.planes * sp / g.splits);
+}
+
+// 32 columns of a warp's 32 rows out, through shared memory so that a row's
+// columns leave together: with one thread per row, as TMEM hands them out,
+// every store of a warp would touch 32 rows.
+__device__ __forceinline__ void store_block(const GemmArgs& g, float* buf, const float* v, int64_t m0, int64_t n0,
+                                            float scale, int sp, int lane) {
+#pragma unroll
+  for (int i = 0; i < 32; i++) buf[lane * kStagePitch + i] = v[i];
+  __syncwarp();
+  const int rows = (int)min((int64_t)32, g.M - m0);
+  const int64_t n = n0 + lane;
+  if (g.splits > 1) {
+    float* d = g.partial + ((int64_t)sp * g.M + m0) * g.N + n;
+    if (n < g.N)
+      for (int r = 0; r < rows; r++) d[r * g.N] = buf[r * kStagePitch + lane];
+  } else if (g.o.dtype != DT_F32 && !g.o.add && n0 + 32 <= g.N &&
+             ((reinterpret_cast<uintptr_t>(g.o.c) | (uintptr_t)(g.o.ld * 2)) & 3u) == 0) {
+    // 16-bit results in pairs, two rows at a time
+    const int c = (lane & 15) * 2;
+    for (int r = lane >> 4; r < rows; r += 2) {
+      const float a = __fmul_rn(buf[r * kStagePitch + c], scale), b = __fmul_rn(buf[r * kStagePitch + c + 1], scale);
+      const uint32_t w = g.o.dtype == DT_F16 ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16
+                                             : f32_to_bf16_bits(a) | (uint32_t)f32_to_bf16_bits(b) << 16;
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(g.o.c) + (m0 + r) * g.o.ld + n0 + c) = w;
+    }
+  } else if (n < g.N) {
+    for (int r = 0; r < rows; r++) finish(g.o, scale, m0 + r, n, buf[r * kStagePitch + lane]);
+  }
+  __syncwarp();
+}
 
 template <bool AMN, bool BMN>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const GemmArgs g) {
   extern __shared__ uint8_t dyn[];
   __shared__ __align__(8) uint64_t bars[2 * kStages + 5];
@@ -255,72 +310,72 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const uint32_t full = sptr(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16,
                  drain = tempty + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   volatile int* abort = &abort_flag;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int i = 0; i < kStages; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; i++) mbar_init(tfull + 8 * i, 1), mbar_init(tempty + 8 * i, 8);
+    for (int i = 0; i < 2; i++) mbar_init(tfull + 8 * i, 1), mbar_init(tempty + 8 * i, 16);
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sptr(&tmem_base)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sptr(&tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_base;
-  const int total = g.steps * g.planes;
   const int units = g.tiles_m * g.tiles_n * g.splits;
-  int issued = 0;  // stages filled (warp 0)
 
   if (warp == 0 && lane == 0) {
-    for (int u = blockIdx.x; u < units && !*abort; u += gridDim.x) {
+    int it = 0;
+    const uint32_t lead = in_cta(full, 0);
+    bool ok = true;
+    for (int u = pair; u < units && ok && !*abort; u += pairs) {
       int tm, tn;
       const int sp = u % g.splits;
       tile_at(g, u / g.splits, tm, tn);
-      const int s0 = (int)((int64_t)total * sp / g.splits), s1 = (int)((int64_t)total * (sp + 1) / g.splits);
-      bool ok = true;
-      for (int s = s0; s < s1; s++) {
-        const int st = issued % kStages;
-        if (issued >= kStages && !(ok = mbar_wait(empty + 8 * st, (issued / kStages - 1) & 1, abort))) break;
-        const uint32_t a = smem + st * kStageBytes, b = a + kABytes, bar = full + 8 * st;
+      const int s1 = split_at(g, sp + 1);
+      const int am = tm * kBM + rank * kHalf, bn = tn * kBN + rank * kHalf;
+      for (int s = split_at(g, sp); s < s1; s++, it++) {
+        const int st = it % kStages;
+        if (it >= kStages && !(ok = mbar_wait(empty + 8 * st, (it / kStages - 1) & 1, abort))) break;
+        const uint32_t a = smem + st * kStageBytes, b = a + kHalfBytes, bar = lead + 8 * st;
         const int p = s / g.steps, r = (s - p * g.steps) * kBK;
-        mbar_expect(bar, kStageBytes);
+        if (rank == 0) mbar_expect(full + 8 * st, 2 * kStageBytes);
         if (AMN) {
 #pragma unroll
-          for (int i = 0; i < kBM / 64; i++) tma_load3(a + i * kBK * 128, &ma, bar, tm * kBM + i * 64, r, p);
+          for (int i = 0; i < kHalf / 64; i++) tma_load3(a + i * kBK * 128, &ma, bar, am + i * 64, r, p);
         } else {
-          tma_load3(a, &ma, bar, r, tm * kBM, p);
+          tma_load3(a, &ma, bar, r, am, p);
         }
         if (BMN) {
 #pragma unroll
-          for (int i = 0; i < kBN / 64; i++) tma_load3(b + i * kBK * 128, &mb, bar, tn * kBN + i * 64, r, 0);
+          for (int i = 0; i < kHalf / 64; i++) tma_load3(b + i * kBK * 128, &mb, bar, bn + i * 64, r, 0);
         } else {
-          tma_load3(b, &mb, bar, r, tn * kBN, 0);
+          tma_load3(b, &mb, bar, r, bn, 0);
         }
-        issued++;
       }
-      if (!ok) break;
     }
-    if (*abort) {  // no copy may still be in flight when the CTA's memory goes
-      for (int i = issued > kStages ? issued - kStages : 0; i < issued; i++) {
+    if (*abort && rank == 0) {  // no copy may still be in flight when the CTAs' memory goes
+      for (int i = it > kStages ? it - kStages : 0; i < it; i++) {
         const unsigned long long t0 = now_ns();
         while (!mbar_try(full + 8 * (i % kStages), (i / kStages) & 1) && now_ns() - t0 < kGemmWaitNs) {
         }
       }
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1 && lane == 0 && rank == 0) {
     // D float32, A and B bfloat16, majors, N, M
     constexpr uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)AMN << 15 | (uint32_t)BMN << 16 |
                                (uint32_t)(kBN >> 3) << 17 | (uint32_t)(kBM >> 4) << 24;
     int it = 0, chunk = 0;
     bool ok = true;
-    for (int u = blockIdx.x; u < units && ok && !*abort; u += gridDim.x) {
-      const int sp = u % g.splits;
-      const int s0 = (int)((int64_t)total * sp / g.splits), s1 = (int)((int64_t)total * (sp + 1) / g.splits);
-      for (int c = s0; c < s1 && ok; c += kChunk64, chunk++) {
+    for (int u = pair; u < units && ok && !*abort; u += pairs) {
+      const int sp = u % g.splits, s1 = split_at(g, sp + 1);
+      for (int c = split_at(g, sp); c < s1 && ok; c += kChunk64, chunk++) {
         const int buf = chunk & 1;
         if (chunk >= 2 && !(ok = mbar_wait(tempty + 8 * buf, (chunk / 2 - 1) & 1, abort))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -329,7 +384,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const int st = it % kStages;
           if (!(ok = mbar_wait(full + 8 * st, (it / kStages) & 1, abort))) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t a = smem + st * kStageBytes, b = a + kABytes;
+          const uint32_t a = smem + st * kStageBytes, b = a + kHalfBytes;
 #pragma unroll
           for (int k = 0; k < kBK / 16; k++)
             mma_f16(tmem + buf * kBN, smem_desc<AMN>(a + k * (AMN ? 2048 : 32)), smem_desc<BMN>(b + k * (BMN ? 2048 : 32)),
@@ -348,18 +403,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   } else if (warp >= 4) {
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + half * (kBN / 2);
+    const uint32_t done = in_cta(tempty, 0);
+    float* buf32 = reinterpret_cast<float*>(dyn + (smem - sptr(dyn)) + kStages * kStageBytes) + (warp - 4) * 32 * kStagePitch;
     const float scale = out_scale(g.o);
     int chunk = 0;
     bool ok = true;
-    for (int u = blockIdx.x; u < units && ok && !*abort; u += gridDim.x) {
+    for (int u = pair; u < units && ok && !*abort; u += pairs) {
       int tm, tn;
-      const int sp = u % g.splits;
+      const int sp = u % g.splits, s1 = split_at(g, sp + 1);
       tile_at(g, u / g.splits, tm, tn);
-      const int s0 = (int)((int64_t)total * sp / g.splits), s1 = (int)((int64_t)total * (sp + 1) / g.splits);
       float acc[kBN / 2];
 #pragma unroll
       for (int i = 0; i < kBN / 2; i++) acc[i] = 0.0f;
-      for (int c = s0; c < s1; c += kChunk64, chunk++) {
+      for (int c = split_at(g, sp); c < s1; c += kChunk64, chunk++) {
         const int buf = chunk & 1;
         if (!(ok = mbar_wait(tfull + 8 * buf, (chunk / 2) & 1, abort))) break;
         __syncwarp();
@@ -378,88 +434,56 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty + 8 * buf);
+        if (lane == 0) mbar_arrive_cluster(done + 8 * buf);
       }
       if (!ok) break;
-      const int64_t m = (int64_t)tm * kBM + quarter * 32 + lane, n0 = (int64_t)tn * kBN + half * (kBN / 2);
-      if (m < g.M) {
-        if (g.splits > 1) {
-          float* d = g.partial + ((int64_t)sp * g.M + m) * g.N;
-          if ((g.N & 3) == 0) {
+      const int64_t m0 = (int64_t)tm * kBM + rank * kHalf + quarter * 32, n0 = (int64_t)tn * kBN + half * (kBN / 2);
 #pragma unroll
-            for (int i = 0; i < kBN / 2; i += 4)
-              if (n0 + i < g.N)
-                *reinterpret_cast<float4*>(d + n0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < kBN / 2; i++)
-              if (n0 + i < g.N) d[n0 + i] = acc[i];
-          }
-        } else {
-          const int64_t at = m * g.o.ld + n0;
-          const int e = g.o.dtype == DT_F32 ? 4 : 2;
-          const bool wide = ((reinterpret_cast<uintptr_t>(g.o.c) | reinterpret_cast<uintptr_t>(g.o.add) |
-                              (uintptr_t)(g.o.ld * e)) & 15u) == 0;
-#pragma unroll
-          for (int i = 0; i < kBN / 2; i += 8) {
-            if (n0 + i >= g.N) break;
-            if (wide && n0 + i + 8 <= g.N) {
-              float v[8];
-#pragma unroll
-              for (int k = 0; k < 8; k++) v[k] = __fmul_rn(acc[i + k], scale);
-              if (g.o.dtype == DT_F32) {
-                if (g.o.add) {
-                  const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(g.o.add) + at + i);
-                  const float4 a = s[0], b = s[1];
-                  const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-                  for (int k = 0; k < 8; k++) v[k] = __fadd_rn(v[k], w[k]);
-                }
-                float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(g.o.c) + at + i);
-                d[0] = make_float4(v[0], v[1], v[2], v[3]);
-                d[1] = make_float4(v[4], v[5], v[6], v[7]);
-              } else {
-                if (g.o.add) {
-                  const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(g.o.add) + at + i);
-                  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                  for (int k = 0; k < 8; k++) {
-                    const uint16_t h = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
-                    v[k] = __fadd_rn(v[k], g.o.dtype == DT_F16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h));
-                  }
-                }
-                uint32_t w[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                  w[k] = g.o.dtype == DT_F16
-                             ? f32_to_f16_bits(v[2 * k]) | (uint32_t)f32_to_f16_bits(v[2 * k + 1]) << 16
-                             : f32_to_bf16_bits(v[2 * k]) | (uint32_t)f32_to_bf16_bits(v[2 * k + 1]) << 16;
-                *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(g.o.c) + at + i) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-            } else {
-#pragma unroll
-              for (int k = 0; k < 8; k++)
-                if (n0 + i + k < g.N) finish(g.o, scale, m, n0 + i + k, acc[i + k]);
-            }
-          }
-        }
-      }
+      for (int i = 0; i < kBN / 2; i += 32)
+        if (m0 < g.M && n0 + i < g.N) store_block(g, buf32, acc + i, m0, n0 + i, scale, sp, lane);
     }
   }
   __syncthreads();
-  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  if (*abort && warp == 0) {  // what the other CTA's copies still do ends in this time
+    const unsigned long long t0 = now_ns();
+    while (now_ns() - t0 < 1000000ull) {
+    }
+  }
+  __syncwarp();
+  cluster_sync();
+  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// the splits' sums, added in their order
+// the splits' sums, added in their order; four columns per thread
 __global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict__ partial, int splits, int64_t M, int64_t N,
                                                         LinearOut o) {
   const float scale = out_scale(o);
-  const int64_t n = M * N, stride = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < n; t += stride) {
-    float v = partial[t];
-    for (int s = 1; s < splits; s++) v = __fadd_rn(v, partial[s * n + t]);
-    const int64_t m = t / N;
-    finish(o, scale, m, t - m * N, v);
+  const int64_t mn = M * N;
+  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+    const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (n >= N) continue;
+    const float* s = partial + m * N + n;
+    float v[4];
+    const int w = (int)min((int64_t)4, N - n);
+    if ((N & 3) == 0) {
+      float4 t = __ldcs(reinterpret_cast<const float4*>(s));
+      v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+      for (int i = 1; i < splits; i++) {
+        t = __ldcs(reinterpret_cast<const float4*>(s + i * mn));
+        v[0] = __fadd_rn(v[0], t.x), v[1] = __fadd_rn(v[1], t.y);
+        v[2] = __fadd_rn(v[2], t.z), v[3] = __fadd_rn(v[3], t.w);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; k++) v[k] = k < w ? s[k] : 0.0f;
+      for (int i = 1; i < splits; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (k < w) v[k] = __fadd_rn(v[k], s[i * mn + k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (k < w) finish(o, scale, m, n + k, v[k]);
   }
 }
 
@@ -534,13 +558,13 @@ Plan make_plan(const LinearArgs& a, int sms) {
   p.steps = (int)((p.R + kBK - 1) / kBK);
   p.tiles_m = (int)((p.M + kBM - 1) / kBM);
   p.tiles_n = (int)((p.N + kBN - 1) / kBN);
-  // fewer tiles than SMs: the reduction is split so that every SM has a part,
-  // of one chunk at least
+  // fewer tiles than pairs of SMs: the reduction is split so that every pair
+  // has a part, of one chunk at least
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, total = (int64_t)p.steps * p.planes;
   p.splits = 1;
-  if (tiles < sms) {
+  if (tiles < sms / 2) {
     const int64_t most = (total + kChunk64 - 1) / kChunk64;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(sms / tiles, most));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(sms / 2 / tiles, most));
   }
   p.q_off = 0;
   p.a_off = up(p.q_off + p.qrows * p.qp * 2, 256);
@@ -576,7 +600,7 @@ cudaError_t run_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArg
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
   const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-  gemm_kernel<AMN, BMN><<<(unsigned)std::min<int64_t>(units, sms), kGemmThreads, kGemmSmem, st>>>(ma, mb, g);
+  gemm_kernel<AMN, BMN><<<(unsigned)std::min<int64_t>(units, sms / 2) * 2, kGemmThreads, kGemmSmem, st>>>(ma, mb, g);
   return cudaGetLastError();
 }
 
@@ -642,8 +666,8 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
   }
   const bool amn = a.op == LIN_WGRAD, bmn = a.op != LIN_FORWARD;
   CUtensorMap ma, mb;
-  if ((e = make_map(&ma, abase, p.acols, p.arows, p.planes, apitch, aplane, amn ? kBK : kBM)) != cudaSuccess) return e;
-  if ((e = make_map(&mb, q16, p.qcols, p.qrows, 1, p.qp, p.qrows * p.qp, bmn ? kBK : kBN)) != cudaSuccess) return e;
+  if ((e = make_map(&ma, abase, p.acols, p.arows, p.planes, apitch, aplane, amn ? kBK : kHalf)) != cudaSuccess) return e;
+  if ((e = make_map(&mb, q16, p.qcols, p.qrows, 1, p.qp, p.qrows * p.qp, bmn ? kBK : kHalf)) != cudaSuccess) return e;
   GemmArgs g;
   g.o = a.o;
   g.M = p.M, g.N = p.N;
@@ -657,7 +681,9 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
   else
     e = run_gemm<true, true>(ma, mb, g, sms, st);
   if (e != cudaSuccess || p.splits == 1) return e;
-  gemm_join_kernel<<<grid_for(p.M * p.N, sms), 256, 0, st>>>(g.partial, p.splits, p.M, p.N, a.o);
+  const int64_t jx = (p.N + 1023) / 1024;
+  gemm_join_kernel<<<dim3((unsigned)jx, (unsigned)std::min<int64_t>(p.M, 65535)), 256, 0, st>>>(g.partial, p.splits, p.M,
+                                                                                               p.N, a.o);
   return cudaGetLastError();
 }
 
