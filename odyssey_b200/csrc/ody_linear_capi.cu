@@ -286,8 +286,8 @@ extern "C" int ody_linear_status(void* stream) {
 }
 
 // Test hook (not part of include/odyssey_mp.h): a device-side wait that runs
-// out after limit_ns.
-extern "C" int odyx_linear_wait_selftest(uint64_t limit_ns, void* stream) {
-  ODY_CUDA(launch_wait_selftest(limit_ns, (cudaStream_t)stream));
+// out after so many cycles.
+extern "C" int odyx_linear_wait_selftest(int64_t cycles, void* stream) {
+  ODY_CUDA(launch_wait_selftest(cycles, (cudaStream_t)stream));
   return ODY_OK;
 }

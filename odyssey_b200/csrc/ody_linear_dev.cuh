@@ -40,6 +40,41 @@ struct W4 {
   }
 };
 
+// ---- eight weights at once, as bfloat16 pairs -------------------------------
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// the block scale as a bfloat16 pair (exact)
+template <int KIND>
+__device__ __forceinline__ uint32_t w4_scale_bf16x2(uint32_t byte) {
+  uint32_t h;
+  if (KIND == Q_MXFP4)
+    h = byte << 7;  // 0 is 0, 255 is infinity
+  else if (KIND == Q_MXFP4_OCP)
+    h = byte == 0xFF ? 0x7fc0u : (byte ? byte << 7 : 0x0040u);
+  else
+    h = __float_as_uint(e4m3_to_f32((uint8_t)byte)) >> 16;
+  return h | h << 16;
+}
+// Four code bytes (eight weights, the first in the lowest byte's high nibble)
+// as o[i] = weights 2i, 2i + 1, times 2^-126: the code's three magnitude bits
+// put where bfloat16 keeps the lowest two exponent bits and the highest
+// mantissa bit (0.5 as a subnormal), its sign on top.  Only the OCP kind has
+// 0.5; in the others that code is zero.
+template <int KIND>
+__device__ __forceinline__ void w4_raw8(uint32_t w, uint32_t o[4]) {
+  if (KIND != Q_MXFP4_OCP) w &= ~0x11111111u | (w >> 1) | (w >> 2);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    // byte i: its high nibble to bits 12..15, its low one to bits 28..31
+    const uint32_t t = ((w >> (8 * i)) & 0xffu) * 0x10000100u;
+    o[i] = (t & 0x80008000u) | ((t >> 6) & 0x01c001c0u);
+  }
+}
+constexpr uint32_t kTwo126 = 0x7e807e80u;  // 2^126 as a bfloat16 pair
+
 template <int FMT>
 __device__ __forceinline__ float a8_value(uint32_t code, uint32_t scale_byte) {
   const float v = FMT == A8_E4M3 ? e4m3_to_f32((uint8_t)code) : e5m2_to_f32((uint8_t)code);

@@ -2,6 +2,7 @@
 // bfloat16 (exactly) once in the workspace, the other one too unless it can
 // be read where it lies, and a tcgen05 kernel multiplies them.
 #include <cuda.h>
+#include <math.h>
 
 #include "ody_linear_dev.cuh"
 #include "ody_linear_gemm.h"
@@ -13,45 +14,41 @@ namespace ody {
 // ---------------------------------------------------------------------------
 
 // Rows of whole blocks: the weight is one flat run of blocks, so are its
-// bfloat16 values.  A tile of 2048 elements is 1152 or 1088 bytes, copied to
-// shared memory with 16-byte loads; every thread decodes eight elements.
+// bfloat16 values.  A tile of 4096 elements is 2304 or 2176 bytes, copied to
+// shared memory with 16-byte loads; every thread then decodes eight elements
+// twice, so that neighbouring threads write neighbouring 16 bytes.
+constexpr int kUnpackTile = 4096;
 template <int KIND>
 __global__ void __launch_bounds__(256) unpack_w4_flat_kernel(const uint8_t* __restrict__ q, int64_t numel,
                                                              uint16_t* __restrict__ out) {
   using W = W4<KIND>;
-  constexpr int TB = 2048 / W::BE * W::SB;
-  __shared__ __align__(16) uint8_t sm[TB + 16];
-  const int64_t bytes = numel / W::BE * W::SB;
-  const int64_t tiles = (numel + 2047) / 2048;
-  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int64_t b0 = t * TB;
-    const int n = (int)(bytes - b0 < TB ? bytes - b0 : TB);
-    const uint8_t* src = q + b0;
-    const int skew = (int)(reinterpret_cast<uintptr_t>(src) & 15u);
-    // 16-byte words that lie wholly inside the tile, single bytes around them
-    const int head = skew ? 16 - skew : 0;
-    for (int i = threadIdx.x; i * 16 + head + 16 <= n; i += 256)
-      *reinterpret_cast<uint4*>(sm + (skew ? 16 : 0) + i * 16) =
-          __ldg(reinterpret_cast<const uint4*>(src + head + i * 16));
-    if ((int)threadIdx.x < head && (int)threadIdx.x < n) sm[skew + threadIdx.x] = src[threadIdx.x];
-    const int rest = head + (n > head ? (n - head) / 16 * 16 : 0);
-    if ((int)threadIdx.x < n - rest) sm[skew + rest + threadIdx.x] = src[rest + threadIdx.x];
-    __syncthreads();
-    const int e = threadIdx.x * 8;
-    if (t * 2048 + e < numel) {
-      const uint8_t* blk = sm + skew + e / W::BE * W::SB;
-      const float sf = W::scale(blk[W::SB - 1]);
-      const uint8_t* c = blk + (e % W::BE) / 2;
-      uint32_t o[4];
+  constexpr int TB = kUnpackTile / W::BE * W::SB;
+  __shared__ __align__(16) uint8_t sm[TB + 32];
+  const int64_t t = blockIdx.x, b0 = t * TB, bytes = numel / W::BE * W::SB;
+  const int n = (int)(bytes - b0 < TB ? bytes - b0 : TB);
+  const uint8_t* src = q + b0;
+  const int skew = (int)(reinterpret_cast<uintptr_t>(src) & 15u);
+  // 16-byte words that lie wholly inside the tile, single bytes around them
+  const int head = skew ? 16 - skew : 0;
+  for (int i = threadIdx.x; i * 16 + head + 16 <= n; i += 256)
+    *reinterpret_cast<uint4*>(sm + (skew ? 16 : 0) + i * 16) = __ldcs(reinterpret_cast<const uint4*>(src + head + i * 16));
+  if ((int)threadIdx.x < head && (int)threadIdx.x < n) sm[skew + threadIdx.x] = src[threadIdx.x];
+  const int rest = head + (n > head ? (n - head) / 16 * 16 : 0);
+  if ((int)threadIdx.x < n - rest) sm[skew + rest + threadIdx.x] = src[rest + threadIdx.x];
+  __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint32_t b = c[i];
-        // the product is exact in bfloat16, so its upper half is all of it
-        o[i] = (__float_as_uint(W::value(b >> 4, sf)) >> 16) | (__float_as_uint(W::value(b & 15u, sf)) & 0xffff0000u);
-      }
-      *reinterpret_cast<uint4*>(out + t * 2048 + e) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    __syncthreads();
+  for (int h = 0; h < kUnpackTile / 2048; h++) {
+    const int e = h * 2048 + threadIdx.x * 8;
+    if (t * kUnpackTile + e >= numel) break;
+    const int blk = skew + e / W::BE * W::SB, at = blk + (e % W::BE) / 2;
+    const uint32_t* wp = reinterpret_cast<const uint32_t*>(sm) + (at >> 2);
+    const uint32_t w = __funnelshift_r(wp[0], wp[1], 8 * (at & 3));
+    const uint32_t sc = w4_scale_bf16x2<KIND>(sm[blk + W::SB - 1]);
+    uint32_t o[4];
+    w4_raw8<KIND>(w, o);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = mul_bf16x2(mul_bf16x2(o[i], kTwo126), sc);
+    *reinterpret_cast<uint4*>(out + t * kUnpackTile + e) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -67,32 +64,32 @@ __global__ void __launch_bounds__(256) unpack_w4_rows_kernel(const uint8_t* __re
     for (int i = 0; i < 4; i++) {
       const float a = c + 2 * i < cols ? W4<KIND>::at(q, r * cols + c + 2 * i) : 0.0f;
       const float b = c + 2 * i + 1 < cols ? W4<KIND>::at(q, r * cols + c + 2 * i + 1) : 0.0f;
+      // the product is exact in bfloat16, so its upper half is all of it
       o[i] = (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xffff0000u);
     }
     *reinterpret_cast<uint4*>(out + r * kp + c) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
-// 8-bit activations: sixteen columns per thread, rows of whole groups.
+// 8-bit activations: eight columns per thread, rows of whole groups.
 template <int FMT>
 __global__ void __launch_bounds__(256) unpack_a8_kernel(const uint8_t* __restrict__ codes,
-                                                        const uint8_t* __restrict__ scales, int64_t n16,
+                                                        const uint8_t* __restrict__ scales, int64_t n8,
                                                         uint16_t* __restrict__ out) {
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < n16; t += stride) {
-    const uint4 c = __ldg(reinterpret_cast<const uint4*>(codes) + t);
-    const uint32_t sb = scales[t >> 1];
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    uint32_t o[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const uint32_t two = w[i >> 1] >> (16 * (i & 1));
+  for (int h = 0; h < 4; h++) {
+    const int64_t t = (int64_t)blockIdx.x * 1024 + h * 256 + threadIdx.x;
+    if (t >= n8) return;
+    const uint2 c = __ldcs(reinterpret_cast<const uint2*>(codes) + t);
+    const uint32_t sb = scales[t >> 2];
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t two = (i < 2 ? c.x : c.y) >> (16 * (i & 1));
       o[i] = (__float_as_uint(a8_value<FMT>(two & 255u, sb)) >> 16) |
              (__float_as_uint(a8_value<FMT>((two >> 8) & 255u, sb)) & 0xffff0000u);
     }
-    uint4* d = reinterpret_cast<uint4*>(out) + 2 * t;
-    d[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    reinterpret_cast<uint4*>(out)[t] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -152,28 +149,38 @@ __global__ void __launch_bounds__(256) pack_planes_kernel(const void* __restrict
 // copied the same way, 64 columns at a time, and multiplied as "MN-major".
 //
 // The tensor core cuts off the low bits of what it adds, so a long sum in one
-// accumulator drifts; every 256 products the accumulator is therefore taken
-// to registers and added there in float32 with rounding, while the tensor
+// accumulator drifts: over 8192 products to a relative 6e-6 (measured), where
+// rounded float32 sums are 2e-7 off.  Every 512 products (1024 where the
+// result is rounded to 16 bits) the accumulator is therefore taken to
+// registers and added there with rounding (3e-7 and 6e-7), while the tensor
 // core fills the other one.
+//
+// Tiles rarely fill a whole number of rounds of the 74 pairs.  Those that do
+// not are dealt out by steps instead, evenly to all pairs, before the whole
+// ones; the pieces of a shared tile are added in their order by gemm_join.
+// (Adding them here, in whichever warp finished last, took 10 to 40 us: eight
+// warps per SM cannot keep enough loads in flight.)
+//
+// A finished block of 32 columns goes through a 32 x 32 transpose in shared
+// memory so that a row's columns leave together; the loop over the blocks is
+// kept rolled (the accumulator moves down by 32 registers instead), because
+// straight-line code is read cold by every launch and cost 11,000 cycles a
+// block.
 // ---------------------------------------------------------------------------
-constexpr int kBM = 256, kBN = 256, kBK = 64, kStages = 6, kChunk64 = 4;
+constexpr int kBM = 256, kBN = 256, kBK = 64, kStages = 6;
 constexpr int kHalf = 128;                                   // rows of A and of B in each CTA
 constexpr int kHalfBytes = kHalf * kBK * 2, kStageBytes = 2 * kHalfBytes;
 constexpr int kStagePitch = 33;                              // floats; the epilogue's 32 x 32 transposes
 constexpr int kEpiBytes = 8 * 32 * kStagePitch * 4;
 constexpr int kGemmSmem = kStages * kStageBytes + kEpiBytes + 1024;
 constexpr int kGemmThreads = 384;
-constexpr unsigned long long kGemmWaitNs = 2000000000ull;  // bound on every wait (2 s)
+// bound on every wait, in cycles of the SM's counter: 2 s at 2 GHz
+constexpr long long kWaitCycles = 4000000000ll;
 
 // set when a bounded wait ran out; read and cleared by gemm_wait_error
 __device__ unsigned g_gemm_err;
 
 __device__ __forceinline__ uint32_t sptr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -186,12 +193,12 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 }
 // false: the wait ran out, or another warp's did
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort,
-                                          unsigned long long limit = kGemmWaitNs) {
+                                          long long limit = kWaitCycles) {
   if (mbar_try(bar, parity)) return true;
-  const unsigned long long t0 = now_ns();
+  const long long t0 = clock64();
   while (!mbar_try(bar, parity)) {
     if (*abort) return false;
-    if (now_ns() - t0 > limit) {
+    if (clock64() - t0 > limit) {
       *abort = 1;
       atomicExch(&g_gemm_err, 1u);
       return false;
@@ -251,10 +258,15 @@ struct GemmArgs {
   LinearOut o;
   int64_t M, N;
   int tiles_m, tiles_n;
-  int steps;         // of 64 of the reduction, per plane
-  int planes;
-  int splits;        // of planes * steps
-  float* partial;    // splits > 1: [splits, M, N]
+  int steps;          // of 64 of the reduction, per plane
+  int total;          // steps * planes: of one tile
+  int chunk;          // steps in one accumulator
+  // The first `shared` tiles' steps are dealt out evenly, `deal` to each pair
+  // of SMs whether or not tiles end there; the other tiles, a multiple of the
+  // number of pairs, go to one pair each.
+  int shared;
+  int deal;
+  float* partial;     // two slots of 256 x 256 per pair: its first and its last piece of a tile, in rows
 };
 
 // tile t's place: bands of eight row tiles, so that CTAs running at once share
@@ -265,39 +277,86 @@ __device__ __forceinline__ void tile_at(const GemmArgs& g, int t, int& tm, int& 
   tm = first + in % h;
   tn = in / h;
 }
-__device__ __forceinline__ int split_at(const GemmArgs& g, int sp) {
-  return (int)((int64_t)g.steps * g.planes * sp / g.splits);
+
+// what a pair of SMs works off, piece by piece
+struct Pieces {
+  int64_t pos, end;  // of the shared tiles' steps
+  int next;          // whole tile
+  int tile, s0, s1;
+  __device__ __forceinline__ Pieces(const GemmArgs& g, int pair) {
+    const int64_t all = (int64_t)g.shared * g.total;
+    pos = min((int64_t)pair * g.deal, all);
+    end = min(pos + g.deal, all);
+    next = g.shared + pair;
+  }
+  __device__ __forceinline__ bool get(const GemmArgs& g, int pairs) {
+    if (pos < end) {
+      tile = (int)(pos / g.total);
+      s0 = (int)(pos - (int64_t)tile * g.total);
+      s1 = (int)min((int64_t)g.total, s0 + (end - pos));
+      pos += s1 - s0;
+      return true;
+    }
+    if (next >= g.tiles_m * g.tiles_n) return false;
+    tile = next, s0 = 0, s1 = g.total;
+    next += pairs;
+    return true;
+  }
+};
+
+// 32 x 32 results (at c, in rows of ld) out of a warp's transposing buffer
+__device__ __forceinline__ void store_block(const float* buf, void* c, const void* add, int dtype, int64_t ld, float scale,
+                                            int rows, int cols, int lane) {
+  const int es = dtype == DT_F32 ? 4 : 2;
+  if (dtype != DT_F32 && !add && cols >= 32 && ((reinterpret_cast<uintptr_t>(c) | (uintptr_t)(ld * 2)) & 3u) == 0) {
+    // 16-bit results in pairs, two rows at a time
+    const int k = (lane & 15) * 2, r0 = lane >> 4;
+    const float* s = buf + r0 * kStagePitch + k;
+    uint16_t* d = reinterpret_cast<uint16_t*>(c) + r0 * ld + k;
+    const bool half = dtype == DT_F16;
+#pragma unroll 4
+    for (int i = r0; i < rows; i += 2, s += 2 * kStagePitch, d += 2 * ld) {
+      const float a = __fmul_rn(s[0], scale), b = __fmul_rn(s[1], scale);
+      *reinterpret_cast<uint32_t*>(d) = half ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16
+                                             : f32_to_bf16_bits(a) | (uint32_t)f32_to_bf16_bits(b) << 16;
+    }
+  } else if (lane < cols) {
+    c = reinterpret_cast<uint8_t*>(c) + lane * es;
+    if (!add && dtype == DT_F32) {
+#pragma unroll 4
+      for (int r = 0; r < rows; r++) reinterpret_cast<float*>(c)[r * ld] = __fmul_rn(buf[r * kStagePitch + lane], scale);
+    } else {
+      // what is added comes in eight rows at a time: one by one, every store
+      // would wait for a load (add may be c, so they are not reordered)
+#pragma unroll 1
+      for (int r = 0; r < rows; r += 8) {
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = add && r + i < rows ? load_elem(add, dtype, (r + i) * ld + lane) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (r + i < rows) {
+            float x = __fmul_rn(buf[(r + i) * kStagePitch + lane], scale);
+            if (add) x = __fadd_rn(x, w[i]);
+            store_elem(c, dtype, (r + i) * ld, x);
+          }
+      }
+    }
+  }
 }
 
-// 32 columns of a warp's 32 rows out, through shared memory so that a row's
-// columns leave together: with one thread per row, as TMEM hands them out,
-// every store of a warp would touch 32 rows.
-__device__ __forceinline__ void store_block(const GemmArgs& g, float* buf, const float* v, int64_t m0, int64_t n0,
-                                            float scale, int sp, int lane) {
-#pragma unroll
-  for (int i = 0; i < 32; i++) buf[lane * kStagePitch + i] = v[i];
-  __syncwarp();
-  const int rows = (int)min((int64_t)32, g.M - m0);
-  const int64_t n = n0 + lane;
-  if (g.splits > 1) {
-    float* d = g.partial + ((int64_t)sp * g.M + m0) * g.N + n;
-    if (n < g.N)
-      for (int r = 0; r < rows; r++) d[r * g.N] = buf[r * kStagePitch + lane];
-  } else if (g.o.dtype != DT_F32 && !g.o.add && n0 + 32 <= g.N &&
-             ((reinterpret_cast<uintptr_t>(g.o.c) | (uintptr_t)(g.o.ld * 2)) & 3u) == 0) {
-    // 16-bit results in pairs, two rows at a time
-    const int c = (lane & 15) * 2;
-    for (int r = lane >> 4; r < rows; r += 2) {
-      const float a = __fmul_rn(buf[r * kStagePitch + c], scale), b = __fmul_rn(buf[r * kStagePitch + c + 1], scale);
-      const uint32_t w = g.o.dtype == DT_F16 ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16
-                                             : f32_to_bf16_bits(a) | (uint32_t)f32_to_bf16_bits(b) << 16;
-      *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(g.o.c) + (m0 + r) * g.o.ld + n0 + c) = w;
-    }
-  } else if (n < g.N) {
-    for (int r = 0; r < rows; r++) finish(g.o, scale, m0 + r, n, buf[r * kStagePitch + lane]);
-  }
-  __syncwarp();
+// tcgen05.ld of 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t v[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr));
 }
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 template <bool AMN, bool BMN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
@@ -328,19 +387,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
   cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_base;
-  const int units = g.tiles_m * g.tiles_n * g.splits;
-
+  // registers: 4 warps x 32 x 64 + 8 x 32 x 216 of the launch's 384 x 168
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0 && lane == 0) {
     int it = 0;
     const uint32_t lead = in_cta(full, 0);
     bool ok = true;
-    for (int u = pair; u < units && ok && !*abort; u += pairs) {
+    Pieces w(g, pair);
+    while (ok && !*abort && w.get(g, pairs)) {
       int tm, tn;
-      const int sp = u % g.splits;
-      tile_at(g, u / g.splits, tm, tn);
-      const int s1 = split_at(g, sp + 1);
+      tile_at(g, w.tile, tm, tn);
       const int am = tm * kBM + rank * kHalf, bn = tn * kBN + rank * kHalf;
-      for (int s = split_at(g, sp); s < s1; s++, it++) {
+      for (int s = w.s0; s < w.s1; s++, it++) {
         const int st = it % kStages;
         if (it >= kStages && !(ok = mbar_wait(empty + 8 * st, (it / kStages - 1) & 1, abort))) break;
         const uint32_t a = smem + st * kStageBytes, b = a + kHalfBytes, bar = lead + 8 * st;
@@ -362,8 +421,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     }
     if (*abort && rank == 0) {  // no copy may still be in flight when the CTAs' memory goes
       for (int i = it > kStages ? it - kStages : 0; i < it; i++) {
-        const unsigned long long t0 = now_ns();
-        while (!mbar_try(full + 8 * (i % kStages), (i / kStages) & 1) && now_ns() - t0 < kGemmWaitNs) {
+        const long long t0 = clock64();
+        while (!mbar_try(full + 8 * (i % kStages), (i / kStages) & 1) && clock64() - t0 < kWaitCycles) {
         }
       }
     }
@@ -373,13 +432,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                                (uint32_t)(kBN >> 3) << 17 | (uint32_t)(kBM >> 4) << 24;
     int it = 0, chunk = 0;
     bool ok = true;
-    for (int u = pair; u < units && ok && !*abort; u += pairs) {
-      const int sp = u % g.splits, s1 = split_at(g, sp + 1);
-      for (int c = split_at(g, sp); c < s1 && ok; c += kChunk64, chunk++) {
+    Pieces w(g, pair);
+    while (ok && !*abort && w.get(g, pairs)) {
+      for (int c = w.s0; c < w.s1 && ok; c += g.chunk, chunk++) {
         const int buf = chunk & 1;
         if (chunk >= 2 && !(ok = mbar_wait(tempty + 8 * buf, (chunk / 2 - 1) & 1, abort))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int ce = min(c + kChunk64, s1);
+        const int ce = min(c + g.chunk, w.s1);
         for (int s = c; s < ce; s++, it++) {
           const int st = it % kStages;
           if (!(ok = mbar_wait(full + 8 * st, (it / kStages) & 1, abort))) break;
@@ -396,11 +455,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     }
     if (*abort) {  // nor an MMA
       mma_commit(drain);
-      const unsigned long long t0 = now_ns();
-      while (!mbar_try(drain, 0) && now_ns() - t0 < kGemmWaitNs) {
+      const long long t0 = clock64();
+      while (!mbar_try(drain, 0) && clock64() - t0 < kWaitCycles) {
       }
     }
-  } else if (warp >= 4) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + half * (kBN / 2);
     const uint32_t done = in_cta(tempty, 0);
@@ -408,29 +469,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     const float scale = out_scale(g.o);
     int chunk = 0;
     bool ok = true;
-    for (int u = pair; u < units && ok && !*abort; u += pairs) {
+    Pieces w(g, pair);
+    while (ok && !*abort && w.get(g, pairs)) {
       int tm, tn;
-      const int sp = u % g.splits, s1 = split_at(g, sp + 1);
-      tile_at(g, u / g.splits, tm, tn);
+      tile_at(g, w.tile, tm, tn);
       float acc[kBN / 2];
 #pragma unroll
       for (int i = 0; i < kBN / 2; i++) acc[i] = 0.0f;
-      for (int c = split_at(g, sp); c < s1; c += kChunk64, chunk++) {
+      for (int c = w.s0; c < w.s1; c += g.chunk, chunk++) {
         const int buf = chunk & 1;
         if (!(ok = mbar_wait(tfull + 8 * buf, (chunk / 2) & 1, abort))) break;
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        // 32 columns are added while the next 32 are on their way
+        uint32_t v[2][32];
+        tmem_load32(taddr + buf * kBN, v[0]);
 #pragma unroll
-        for (int j = 0; j < kBN / 2; j += 16) {
-          uint32_t v[16];
-          asm volatile(
-              "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-              : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-              : "r"(taddr + buf * kBN + j));
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        for (int j = 0; j < kBN / 2; j += 32) {
+          tmem_wait();
+          if (j + 32 < kBN / 2) tmem_load32(taddr + buf * kBN + j + 32, v[(j / 32 + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 16; i++) acc[j + i] = __fadd_rn(acc[j + i], __uint_as_float(v[i]));
+          for (int i = 0; i < 32; i++) acc[j + i] = __fadd_rn(acc[j + i], __uint_as_float(v[(j / 32) & 1][i]));
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
@@ -438,15 +497,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
       }
       if (!ok) break;
       const int64_t m0 = (int64_t)tm * kBM + rank * kHalf + quarter * 32, n0 = (int64_t)tn * kBN + half * (kBN / 2);
+      if (m0 >= g.M || n0 >= g.N) continue;
+      void* c;
+      const void* add = nullptr;
+      int dtype = DT_F32;
+      int64_t ld = kBN;
+      float sc = 1.0f;
+      if (w.s1 - w.s0 < g.total) {  // a piece of a shared tile
+        c = g.partial + (int64_t)(2 * pair + (w.s0 == 0)) * kBM * kBN + (rank * kHalf + quarter * 32) * kBN + half * (kBN / 2);
+      } else {
+        dtype = g.o.dtype, ld = g.o.ld, sc = scale;
+        const int64_t at = (m0 * ld + n0) * (dtype == DT_F32 ? 4 : 2);
+        c = reinterpret_cast<uint8_t*>(g.o.c) + at;
+        if (g.o.add) add = reinterpret_cast<const uint8_t*>(g.o.add) + at;
+      }
+      const int rows = (int)min((int64_t)32, g.M - m0), es = dtype == DT_F32 ? 4 : 2;
+      int cols = (int)min((int64_t)(kBN / 2), g.N - n0);
+#pragma unroll 1
+      for (; cols > 0; cols -= 32) {
 #pragma unroll
-      for (int i = 0; i < kBN / 2; i += 32)
-        if (m0 < g.M && n0 + i < g.N) store_block(g, buf32, acc + i, m0, n0 + i, scale, sp, lane);
+        for (int i = 0; i < 32; i++) buf32[lane * kStagePitch + i] = acc[i];
+#pragma unroll
+        for (int i = 0; i < kBN / 2 - 32; i++) acc[i] = acc[i + 32];
+        __syncwarp();
+        store_block(buf32, c, add, dtype, ld, sc, rows, cols, lane);
+        __syncwarp();
+        c = reinterpret_cast<uint8_t*>(c) + 32 * es;
+        if (add) add = reinterpret_cast<const uint8_t*>(add) + 32 * es;
+      }
     }
   }
   __syncthreads();
   if (*abort && warp == 0) {  // what the other CTA's copies still do ends in this time
-    const unsigned long long t0 = now_ns();
-    while (now_ns() - t0 < 1000000ull) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000) {
     }
   }
   __syncwarp();
@@ -454,41 +538,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// the splits' sums, added in their order; four columns per thread
-__global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict__ partial, int splits, int64_t M, int64_t N,
-                                                        LinearOut o) {
-  const float scale = out_scale(o);
-  const int64_t mn = M * N;
-  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
-    const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (n >= N) continue;
-    const float* s = partial + m * N + n;
-    float v[4];
-    const int w = (int)min((int64_t)4, N - n);
-    if ((N & 3) == 0) {
-      float4 t = __ldcs(reinterpret_cast<const float4*>(s));
-      v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-      for (int i = 1; i < splits; i++) {
-        t = __ldcs(reinterpret_cast<const float4*>(s + i * mn));
-        v[0] = __fadd_rn(v[0], t.x), v[1] = __fadd_rn(v[1], t.y);
-        v[2] = __fadd_rn(v[2], t.z), v[3] = __fadd_rn(v[3], t.w);
-      }
-    } else {
+// The shared tiles' results: their pieces added in the order of the steps.  64
+// threads per row with four columns each, eight rows per CTA.
+__global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs g) {
+  const int tile = blockIdx.x >> 5;
+  int tm, tn;
+  tile_at(g, tile, tm, tn);
+  const int64_t t0 = (int64_t)tile * g.total;
+  const int first = (int)(t0 / g.deal), last = (int)((t0 + g.total - 1) / g.deal);
+  if (first == last) return;  // a whole tile
+  const float scale = out_scale(g.o);
+  const int c = (threadIdx.x & 63) * 4;
+  const int64_t n = (int64_t)tn * kBN + c;
+  if (n >= g.N) return;
+  const int w = (int)min((int64_t)4, g.N - n);
 #pragma unroll
-      for (int k = 0; k < 4; k++) v[k] = k < w ? s[k] : 0.0f;
-      for (int i = 1; i < splits; i++)
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (k < w) v[k] = __fadd_rn(v[k], s[i * mn + k]);
+  for (int h = 0; h < 2; h++) {
+    const int r = (blockIdx.x & 31) * 8 + h * 4 + (threadIdx.x >> 6);
+    const int64_t m = (int64_t)tm * kBM + r;
+    if (m >= g.M) return;
+    const float* s = g.partial + r * kBN + c;
+    float4 v = *reinterpret_cast<const float4*>(s + (int64_t)(2 * first + ((int64_t)first * g.deal <= t0)) * kBM * kBN);
+#pragma unroll 4
+    for (int q = first + 1; q <= last; q++) {
+      const float4 f = *reinterpret_cast<const float4*>(s + (int64_t)(2 * q) * kBM * kBN);  // begins inside the tile
+      v.x = __fadd_rn(v.x, f.x), v.y = __fadd_rn(v.y, f.y), v.z = __fadd_rn(v.z, f.z), v.w = __fadd_rn(v.w, f.w);
     }
+    const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int k = 0; k < 4; k++)
-      if (k < w) finish(o, scale, m, n + k, v[k]);
+      if (k < w) finish(g.o, scale, m, n + k, x[k]);
   }
 }
 
 // A wait for a barrier that nothing arrives at (the time-out path's test).
-__global__ void wait_selftest_kernel(unsigned long long limit) {
+__global__ void wait_selftest_kernel(long long limit) {
   __shared__ __align__(8) uint64_t bar;
   __shared__ int abort_flag;
   abort_flag = 0;
@@ -539,7 +623,8 @@ struct Plan {
   int64_t M, N, R;              // the product's
   int64_t qrows, qcols, qp;     // the quantised operand as bfloat16, pitch qp
   int64_t arows, acols, ap;     // the other one, pitch of its planes ap
-  int planes, steps, tiles_m, tiles_n, splits;
+  int planes, steps, tiles_m, tiles_n, shared, deal;
+  bool split;  // some tile is shared by several pairs
   int64_t q_off, a_off, p_off, bytes;
 };
 
@@ -558,18 +643,20 @@ Plan make_plan(const LinearArgs& a, int sms) {
   p.steps = (int)((p.R + kBK - 1) / kBK);
   p.tiles_m = (int)((p.M + kBM - 1) / kBM);
   p.tiles_n = (int)((p.N + kBN - 1) / kBN);
-  // fewer tiles than pairs of SMs: the reduction is split so that every pair
-  // has a part, of one chunk at least
+  // Tiles that do not fill a whole round of the pairs are dealt out by steps.
+  // A tile is shared by about sqrt(total) / 2 pairs at most: a piece costs
+  // about as long as four steps take.
+  const int pairs = sms / 2;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n, total = (int64_t)p.steps * p.planes;
-  p.splits = 1;
-  if (tiles < sms / 2) {
-    const int64_t most = (total + kChunk64 - 1) / kChunk64;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(sms / 2 / tiles, most));
-  }
+  const int64_t shared = tiles % pairs;
+  const int64_t most = std::max<int64_t>(1, (int64_t)(sqrt((double)total) / 2));
+  int64_t deal = std::max((shared * total + pairs - 1) / pairs, (total + most - 1) / most);
+  p.shared = (int)shared, p.deal = (int)std::max<int64_t>(deal, 1);
+  p.split = shared > 0 && deal % total != 0;
   p.q_off = 0;
   p.a_off = up(p.q_off + p.qrows * p.qp * 2, 256);
   p.p_off = up(p.a_off + p.planes * p.arows * p.ap * 2, 256);
-  p.bytes = p.p_off + (p.splits > 1 ? up((int64_t)p.splits * p.M * p.N * 4, 256) : 0);
+  p.bytes = p.p_off + (p.split ? (int64_t)pairs * 2 * kBM * kBN * 4 : 0);
   return p;
 }
 
@@ -581,9 +668,11 @@ template <int KIND>
 cudaError_t unpack_w4(const LinearArgs& a, const Plan& p, uint16_t* out, int sms, cudaStream_t st) {
   if (a.in % W4<KIND>::BE == 0) {
     const int64_t n = a.out * a.in;
-    unpack_w4_flat_kernel<KIND><<<grid_for(n / 8, sms), 256, 0, st>>>(a.q, n, out);
+    unpack_w4_flat_kernel<KIND>
+        <<<(unsigned)((n + kUnpackTile - 1) / kUnpackTile), 256, 0, st>>>(a.q, n, out);
   } else {
-    unpack_w4_rows_kernel<KIND><<<grid_for(p.qrows * p.qp / 8, sms), 256, 0, st>>>(a.q, p.qrows, p.qcols, p.qp, out);
+    unpack_w4_rows_kernel<KIND>
+        <<<grid_for(p.qrows * p.qp / 8, sms), 256, 0, st>>>(a.q, p.qrows, p.qcols, p.qp, out);
   }
   return cudaGetLastError();
 }
@@ -599,8 +688,10 @@ cudaError_t run_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArg
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
-  const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-  gemm_kernel<AMN, BMN><<<(unsigned)std::min<int64_t>(units, sms / 2) * 2, kGemmThreads, kGemmSmem, st>>>(ma, mb, g);
+  // with whole tiles only, no more pairs than tiles
+  const int64_t shares = ((int64_t)g.shared * g.total + g.deal - 1) / g.deal;
+  const int64_t work = g.tiles_m * (int64_t)g.tiles_n > g.shared ? sms / 2 : shares;
+  gemm_kernel<AMN, BMN><<<(unsigned)std::min<int64_t>(work, sms / 2) * 2, kGemmThreads, kGemmSmem, st>>>(ma, mb, g);
   return cudaGetLastError();
 }
 
@@ -619,8 +710,8 @@ cudaError_t gemm_wait_error(cudaStream_t st, bool* ran_out) {
   return e;
 }
 
-cudaError_t launch_wait_selftest(unsigned long long limit_ns, cudaStream_t st) {
-  wait_selftest_kernel<<<1, 1, 0, st>>>(limit_ns);
+cudaError_t launch_wait_selftest(long long cycles, cudaStream_t st) {
+  wait_selftest_kernel<<<1, 1, 0, st>>>(cycles);
   return cudaGetLastError();
 }
 
@@ -632,11 +723,12 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
   uint16_t* q16 = reinterpret_cast<uint16_t*>(base + p.q_off);
   cudaError_t e;
   if (a.op == LIN_WGRAD) {
-    const int64_t n16 = p.qrows * p.qp / 16;
+    const int64_t n8 = p.qrows * p.qp / 8;
+    const unsigned grid = (unsigned)((n8 + 1023) / 1024);
     if (a.kind == A8_E4M3)
-      unpack_a8_kernel<A8_E4M3><<<grid_for(n16, sms), 256, 0, st>>>(a.q, a.scales, n16, q16);
+      unpack_a8_kernel<A8_E4M3><<<grid, 256, 0, st>>>(a.q, a.scales, n8, q16);
     else
-      unpack_a8_kernel<A8_E5M2><<<grid_for(n16, sms), 256, 0, st>>>(a.q, a.scales, n16, q16);
+      unpack_a8_kernel<A8_E5M2><<<grid, 256, 0, st>>>(a.q, a.scales, n8, q16);
     e = cudaGetLastError();
   } else if (a.kind == Q_MXFP4) {
     e = unpack_w4<Q_MXFP4>(a, p, q16, sms, st);
@@ -672,7 +764,8 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
   g.o = a.o;
   g.M = p.M, g.N = p.N;
   g.tiles_m = p.tiles_m, g.tiles_n = p.tiles_n;
-  g.steps = p.steps, g.planes = p.planes, g.splits = p.splits;
+  g.steps = p.steps, g.total = p.steps * p.planes, g.chunk = a.o.dtype == DT_F32 ? 8 : 16;
+  g.shared = p.shared, g.deal = p.deal;
   g.partial = reinterpret_cast<float*>(base + p.p_off);
   if (a.op == LIN_FORWARD)
     e = run_gemm<false, false>(ma, mb, g, sms, st);
@@ -680,10 +773,8 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
     e = run_gemm<false, true>(ma, mb, g, sms, st);
   else
     e = run_gemm<true, true>(ma, mb, g, sms, st);
-  if (e != cudaSuccess || p.splits == 1) return e;
-  const int64_t jx = (p.N + 1023) / 1024;
-  gemm_join_kernel<<<dim3((unsigned)jx, (unsigned)std::min<int64_t>(p.M, 65535)), 256, 0, st>>>(g.partial, p.splits, p.M,
-                                                                                               p.N, a.o);
+  if (e != cudaSuccess || !p.split) return e;
+  gemm_join_kernel<<<(unsigned)p.shared * 32, 256, 0, st>>>(g);
   return cudaGetLastError();
 }
 

@@ -11,5 +11,5 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
 // whether a bounded wait of the current device's kernels ran out since the
 // last call; waits for the device's work on `st`
 cudaError_t gemm_wait_error(cudaStream_t st, bool* ran_out);
-cudaError_t launch_wait_selftest(unsigned long long limit_ns, cudaStream_t st);
+cudaError_t launch_wait_selftest(long long cycles, cudaStream_t st);
 }  // namespace ody
