@@ -16,9 +16,9 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libodyssey_mp.so")
 SOURCES = ["ody_kernels.cu", "ody_capi.cu", "ody_noalloc.cu", "ody_linear.cu", "ody_linear_gemm.cu",
-           "ody_linear_capi.cu"]
+           "ody_linear_rows.cu", "ody_linear_capi.cu"]
 HEADERS = ["ody_internal.h", "ody_numerics.cuh", "ody_fp4fast.cuh", "ody_host.h", "ody_linear.h",
-           "ody_linear_dev.cuh", "ody_linear_gemm.h"]
+           "ody_linear_dev.cuh", "ody_linear_gemm.h", "ody_linear_rows.h"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVFLAGS = ARCH + [

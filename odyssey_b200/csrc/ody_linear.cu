@@ -12,6 +12,7 @@
 #include "ody_linear.h"
 #include "ody_linear_dev.cuh"
 #include "ody_linear_gemm.h"
+#include "ody_linear_rows.h"
 
 namespace ody {
 
@@ -116,9 +117,13 @@ static int lin_sms() {
 // cores, after their operands have been brought to bfloat16.
 static bool small_product(const LinearArgs& a) { return (double)a.rows * a.out * a.in <= 0; }
 
-int64_t linear_workspace(const LinearArgs& a) { return small_product(a) ? 0 : gemm_workspace(a, lin_sms()); }
+// (of any kind: the query does not name one, so widths are taken to be in 32s)
+int64_t linear_workspace(const LinearArgs& a) {
+  return small_product(a) || (few_rows(a) && a.in % 32 == 0) ? 0 : gemm_workspace(a, lin_sms());
+}
 
 cudaError_t launch_linear(const LinearArgs& a, void* ws, cudaStream_t st) {
+  if (few_rows(a)) return launch_few_rows(a, lin_sms(), st);
   if (!small_product(a)) return launch_gemm(a, ws, lin_sms(), st);
   if (a.op == LIN_FORWARD) return launch_fp32_w4<LIN_FORWARD>(a, st);
   if (a.op == LIN_DGRAD) return launch_fp32_w4<LIN_DGRAD>(a, st);
