@@ -80,9 +80,17 @@ int on_stream(const LinearArgs& a, void* ws, size_t ws_bytes, void* stream, cons
   const int64_t need = linear_workspace(a);
   if (need > 0 && (!ws || (int64_t)ws_bytes < need))
     return fail(ODY_ERR_ARG, std::string(name) + ": needs " + std::to_string(need) + " bytes of workspace");
-  if (!is_device_ptr(a.a) || !is_device_ptr(a.q) || (a.scales && !is_device_ptr(a.scales)) || !is_device_ptr(a.o.c) ||
-      (a.o.tscale && !is_device_ptr(a.o.tscale)) || (a.o.add && !is_device_ptr(a.o.add)) ||
-      (need > 0 && !is_device_ptr(ws)))
+  int cur = 0;
+  cudaGetDevice(&cur);
+  const void* const ptrs[] = {a.a, a.q, a.o.c, a.scales, a.o.tscale, a.o.add == a.o.c ? nullptr : a.o.add,
+                              need > 0 ? ws : nullptr};
+  bool here = true;
+  for (const void* p : ptrs)
+    if (p) {
+      const int d = device_of(p);
+      here = here && (d == cur || d == INT32_MAX);
+    }
+  if (!here)
     return fail(ODY_ERR_ARG, std::string(name) + " takes memory of the current GPU only");
   if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 255u))
     return fail(ODY_ERR_ARG, std::string(name) + ": the workspace must be 256-byte aligned");

@@ -9,6 +9,13 @@
 
 namespace ody {
 
+// The kernels of one call follow each other as programmatic dependents: each
+// is set up while the one before it still runs, and waits (previous_done)
+// before it touches what that one wrote.  Every one of them waits, so that
+// the end of the last means the end of all.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void previous_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------
 // Bringing operands to bfloat16
 // ---------------------------------------------------------------------------
@@ -24,6 +31,7 @@ __global__ void __launch_bounds__(256) unpack_w4_flat_kernel(const uint8_t* __re
   using W = W4<KIND>;
   constexpr int TB = kUnpackTile / W::BE * W::SB;
   __shared__ __align__(16) uint8_t sm[TB + 32];
+  let_next_start();
   const int64_t t = blockIdx.x, b0 = t * TB, bytes = numel / W::BE * W::SB;
   const int n = (int)(bytes - b0 < TB ? bytes - b0 : TB);
   const uint8_t* src = q + b0;
@@ -56,6 +64,7 @@ __global__ void __launch_bounds__(256) unpack_w4_flat_kernel(const uint8_t* __re
 template <int KIND>
 __global__ void __launch_bounds__(256) unpack_w4_rows_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols,
                                                              int64_t kp, uint16_t* __restrict__ out) {
+  let_next_start();
   const int64_t n = rows * (kp / 8), stride = (int64_t)gridDim.x * blockDim.x;
   for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < n; t += stride) {
     const int64_t r = t / (kp / 8), c = (t - r * (kp / 8)) * 8;
@@ -76,6 +85,7 @@ template <int FMT>
 __global__ void __launch_bounds__(256) unpack_a8_kernel(const uint8_t* __restrict__ codes,
                                                         const uint8_t* __restrict__ scales, int64_t n8,
                                                         uint16_t* __restrict__ out) {
+  let_next_start();
 #pragma unroll
   for (int h = 0; h < 4; h++) {
     const int64_t t = (int64_t)blockIdx.x * 1024 + h * 256 + threadIdx.x;
@@ -99,6 +109,8 @@ __global__ void __launch_bounds__(256) pack_planes_kernel(const void* __restrict
                                                           int64_t ldx, int64_t cp, int64_t plane, uint16_t* __restrict__ out,
                                                           int wide) {
   constexpr int P = bf16_parts(DT);
+  let_next_start();
+  previous_done();
   const int64_t n = rows * (cp / 8), stride = (int64_t)gridDim.x * blockDim.x;
   for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < n; t += stride) {
     const int64_t r = t / (cp / 8), c = (t - r * (cp / 8)) * 8, at = r * ldx + c;
@@ -387,6 +399,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
   cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_base;
+  let_next_start();
+  previous_done();
   // registers: 4 warps x 32 x 64 + 8 x 32 x 216 of the launch's 384 x 168
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -541,6 +555,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 // The shared tiles' results: their pieces added in the order of the steps.  64
 // threads per row with four columns each, eight rows per CTA.
 __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs g) {
+  previous_done();
   const int tile = blockIdx.x >> 5;
   int tm, tn;
   tile_at(g, tile, tm, tn);
@@ -564,10 +579,37 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs g) {
       const float4 f = *reinterpret_cast<const float4*>(s + (int64_t)(2 * q) * kBM * kBN);  // begins inside the tile
       v.x = __fadd_rn(v.x, f.x), v.y = __fadd_rn(v.y, f.y), v.z = __fadd_rn(v.z, f.z), v.w = __fadd_rn(v.w, f.w);
     }
-    const float x[4] = {v.x, v.y, v.z, v.w};
+    float x[4] = {v.x, v.y, v.z, v.w};
+    const int es = g.o.dtype == DT_F32 ? 4 : 2;
+    const int64_t at = m * g.o.ld + n;
+    if (w == 4 && ((reinterpret_cast<uintptr_t>(g.o.c) | reinterpret_cast<uintptr_t>(g.o.add) | (uintptr_t)(g.o.ld * es)) &
+                   (uintptr_t)(4 * es - 1)) == 0) {  // four results together
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-      if (k < w) finish(g.o, scale, m, n + k, x[k]);
+      for (int k = 0; k < 4; k++) x[k] = __fmul_rn(x[k], scale);
+      if (es == 4) {
+        if (g.o.add) {
+          const float4 f = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(g.o.add) + at);
+          x[0] = __fadd_rn(x[0], f.x), x[1] = __fadd_rn(x[1], f.y), x[2] = __fadd_rn(x[2], f.z), x[3] = __fadd_rn(x[3], f.w);
+        }
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(g.o.c) + at) = make_float4(x[0], x[1], x[2], x[3]);
+      } else {
+        const bool half = g.o.dtype == DT_F16;
+        if (g.o.add) {
+          const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(g.o.add) + at);
+          const uint16_t f[4] = {(uint16_t)u.x, (uint16_t)(u.x >> 16), (uint16_t)u.y, (uint16_t)(u.y >> 16)};
+#pragma unroll
+          for (int k = 0; k < 4; k++) x[k] = __fadd_rn(x[k], half ? f16_bits_to_f32(f[k]) : bf16_bits_to_f32(f[k]));
+        }
+        uint32_t u[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) u[k] = half ? f32_to_f16_bits(x[k]) : f32_to_bf16_bits(x[k]);
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(g.o.c) + at) = make_uint2(u[0] | u[1] << 16, u[2] | u[3] << 16);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (k < w) finish(g.o, scale, m, n + k, x[k]);
+    }
   }
 }
 
@@ -664,6 +706,21 @@ int grid_for(int64_t threads, int sms) {
   return (int)std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, (int64_t)sms * 8));
 }
 
+// a kernel that may be set up while the one before it in the stream runs
+template <class... P, class... A>
+cudaError_t launch_next(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 template <int KIND>
 cudaError_t unpack_w4(const LinearArgs& a, const Plan& p, uint16_t* out, int sms, cudaStream_t st) {
   if (a.in % W4<KIND>::BE == 0) {
@@ -691,8 +748,8 @@ cudaError_t run_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArg
   // with whole tiles only, no more pairs than tiles
   const int64_t shares = ((int64_t)g.shared * g.total + g.deal - 1) / g.deal;
   const int64_t work = g.tiles_m * (int64_t)g.tiles_n > g.shared ? sms / 2 : shares;
-  gemm_kernel<AMN, BMN><<<(unsigned)std::min<int64_t>(work, sms / 2) * 2, kGemmThreads, kGemmSmem, st>>>(ma, mb, g);
-  return cudaGetLastError();
+  return launch_next(gemm_kernel<AMN, BMN>, dim3((unsigned)std::min<int64_t>(work, sms / 2) * 2), kGemmThreads, kGemmSmem,
+                     st, ma, mb, g);
 }
 
 }  // namespace
@@ -748,12 +805,12 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
     apitch = p.ap, aplane = p.arows * p.ap;
     const int grid = grid_for(p.arows * p.ap / 8, sms);
     if (a.a_dtype == DT_F32)
-      pack_planes_kernel<DT_F32><<<grid, 256, 0, st>>>(a.a, p.arows, p.acols, a.lda, apitch, aplane, a16, wide);
+      e = launch_next(pack_planes_kernel<DT_F32>, grid, 256, 0, st, a.a, p.arows, p.acols, a.lda, apitch, aplane, a16, wide);
     else if (a.a_dtype == DT_F16)
-      pack_planes_kernel<DT_F16><<<grid, 256, 0, st>>>(a.a, p.arows, p.acols, a.lda, apitch, aplane, a16, wide);
+      e = launch_next(pack_planes_kernel<DT_F16>, grid, 256, 0, st, a.a, p.arows, p.acols, a.lda, apitch, aplane, a16, wide);
     else
-      pack_planes_kernel<DT_BF16><<<grid, 256, 0, st>>>(a.a, p.arows, p.acols, a.lda, apitch, aplane, a16, wide);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+      e = launch_next(pack_planes_kernel<DT_BF16>, grid, 256, 0, st, a.a, p.arows, p.acols, a.lda, apitch, aplane, a16, wide);
+    if (e != cudaSuccess) return e;
     abase = a16;
   }
   const bool amn = a.op == LIN_WGRAD, bmn = a.op != LIN_FORWARD;
@@ -774,8 +831,7 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
   else
     e = run_gemm<true, true>(ma, mb, g, sms, st);
   if (e != cudaSuccess || !p.split) return e;
-  gemm_join_kernel<<<(unsigned)p.shared * 32, 256, 0, st>>>(g);
-  return cudaGetLastError();
+  return launch_next(gemm_join_kernel, dim3((unsigned)p.shared * 32), 256, 0, st, g);
 }
 
 }  // namespace ody

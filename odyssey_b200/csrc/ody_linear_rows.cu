@@ -500,6 +500,10 @@ cudaError_t launch_rows(const RowArgs& a, int64_t tiles, bool walked, int64_t st
   // CTA still has a step for its warps
   int cluster = 1;
   while (cluster < 8 && tiles * cluster * 2 <= 2 * sms && cluster < steps) cluster *= 2;
+  if (cluster == 1) {
+    kernel<<<(unsigned)(walked ? std::min<int64_t>(tiles, 2 * sms) : tiles), kRowThreads, smem, st>>>(a);
+    return cudaGetLastError();
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((walked ? std::min<int64_t>(tiles, 2 * sms) : tiles) * cluster));
   cfg.blockDim = dim3(kRowThreads);

@@ -18,6 +18,7 @@ dtype='bfloat16') are staged and the call returns when done.
 """
 import ctypes as C
 from dataclasses import dataclass
+from functools import lru_cache
 
 import numpy as np
 
@@ -27,8 +28,8 @@ from .quant import QuantizedTensor
 FORMATS8 = {"e4m3": L.A8_E4M3, "e5m2": L.A8_E5M2}
 _NAMES = ("float32", "float16", "bfloat16")
 _CODES = {"float32": L.F32, "float16": L.F16, "bfloat16": L.BF16, L.F32: L.F32, L.F16: L.F16, L.BF16: L.BF16}
-_W4 = (L.Q_MXFP4, L.Q_NVFP4, L.Q_NVFP4_TENSOR, L.Q_MXFP4_OCP)
-_TORCH = {}
+_BLOCK = {L.Q_MXFP4: (32, 17), L.Q_NVFP4: (16, 9), L.Q_NVFP4_TENSOR: (16, 9), L.Q_MXFP4_OCP: (32, 17)}
+_TORCH = {}  # torch dtype -> code and back, once torch is there
 
 
 def _torch_dtypes():
@@ -66,17 +67,16 @@ class Activation8:
             raise L.OdysseyError(f"unknown 8-bit activation format {self.format!r}", L.ERR_ARG)
         if self.rows <= 0 or self.cols <= 0:
             raise L.OdysseyError("cannot save an empty activation", L.ERR_SHAPE)
-        if L.numel(self.codes) != self.rows * g * 32 or L.numel(self.scales) != self.rows * g:
-            raise L.OdysseyError("codes and scales do not have the bytes of the activation's rows and columns",
-                                 L.ERR_SHAPE)
-        for b in (self.codes, self.scales):
+        for b, n in ((self.codes, self.rows * g * 32), (self.scales, self.rows * g)):
+            if L.numel(b) != n:
+                raise L.OdysseyError("codes and scales do not have the bytes of the activation's rows and columns",
+                                     L.ERR_SHAPE)
             if (b.dtype.itemsize if L.is_torch(b) else np.asarray(b).itemsize) != 1:
                 raise L.OdysseyError("codes and scales must be uint8", L.ERR_DTYPE)
 
 
 class _Rows:
-    """An array as rows of its last axis: the code of its type, pitch, and
-    (for CUDA tensors) the device and torch's current stream on it."""
+    """An array as rows of its last axis: the code of its type and its pitch."""
     __slots__ = ("a", "code", "rows", "cols", "ld", "cuda", "ptr", "lead")
 
     def __init__(self, x, dtype, what):
@@ -88,12 +88,15 @@ class _Rows:
             if len(shape) == 0 or x.numel() == 0:
                 raise L.OdysseyError(f"{what} is empty", L.ERR_SHAPE)
             self.cuda = x.is_cuda
-            if x.dim() != 2:
+            if len(shape) != 2:
                 x = x.reshape(-1, shape[-1])
+            rows, cols = x.shape
+            ld, step = x.stride()
             # rows of any pitch are read in place; anything else is copied
-            if x.stride(1) != 1 and x.shape[1] > 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1] or not self.cuda:
+            if (step != 1 and cols > 1) or (rows > 1 and ld < cols) or not self.cuda:
                 x = x.contiguous()
-            self.ld = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+                ld = cols
+            self.ld = ld if rows > 1 else cols
             self.ptr = x.data_ptr()
         else:
             code = L.dtype_code(x, dtype)
@@ -103,17 +106,22 @@ class _Rows:
                 raise L.OdysseyError(f"{what} is empty", L.ERR_SHAPE)
             self.cuda = False
             x = x.reshape(-1, shape[-1])
-            self.ld = x.shape[1]
+            rows, cols = x.shape
+            self.ld = cols
             self.ptr = x.ctypes.data
-        self.a, self.code, self.lead = x, code, tuple(shape[:-1])
-        self.rows, self.cols = x.shape
+        self.a, self.code, self.lead, self.rows, self.cols = x, code, shape[:-1], rows, cols
+
+
+class _Place:
+    """Where a buffer lies (what _same_place and _out ask of _Rows)."""
+
+    def __init__(self, a):
+        self.a, self.cuda = a, L.is_torch(a) and a.is_cuda
 
 
 def _same_place(x, *others):
     """Buffers of one call live on one device (or all on the host)."""
     for o in others:
-        if o is None:
-            continue
         t = L.is_torch(o) and o.is_cuda
         if t != x.cuda or (t and o.device != x.a.device):
             raise L.OdysseyError("the buffers of a call must be on one device", L.ERR_ARG)
@@ -123,7 +131,7 @@ def _out(x, out, shape, code, what):
     """The result buffer: new, or the caller's after its checks."""
     if out is None:
         if L.is_torch(x.a):
-            return L._torch().empty(shape, dtype=_torch_dtypes()[code], device=x.a.device)
+            return x.a.new_empty(shape, dtype=_torch_dtypes()[code])
         return np.empty(shape, (np.float32, np.float16, np.uint16)[code])
     _same_place(x, out)
     have = _torch_dtypes().get(out.dtype) if L.is_torch(out) else \
@@ -136,34 +144,38 @@ def _out(x, out, shape, code, what):
     return out
 
 
-class _On:
-    """The device of a CUDA call made current, and torch's stream on it."""
-
-    def __init__(self, device):
-        t = L._torch()
-        self.guard = t.cuda.device(device) if device.index != t.cuda.current_device() else None
-        self.device = device
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return L._torch().cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _flat(a):
+    return a if a.is_contiguous() else a.contiguous()
 
 
-def _workspace(op, rows, out, inn, code, device):
-    n = L.lib().ody_linear_workspace(op, rows, out, inn, code)
+def _enqueue(device, call):
+    """call(stream) with the device current and torch's stream on it; raises
+    on a non-zero status."""
+    t = L._torch()
+    index = device.index
+    if index != t.cuda.current_device():
+        with t.cuda.device(index):
+            return L.check(call(t.cuda.current_stream(index).cuda_stream))
+    raw = getattr(t._C, "_cuda_getCurrentRawStream", None)  # the handle without a Stream object around it
+    return L.check(call(raw(index) if raw is not None else t.cuda.current_stream(index).cuda_stream))
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(device_index, op, rows, out, inn, code):
+    return int(L.lib().ody_linear_workspace(op, rows, out, inn, code))
+
+
+def _workspace(a, op, rows, out, inn, code):
+    """(tensor or None, its address, its bytes) for one call on a's device."""
+    n = _workspace_bytes(a.device.index, op, rows, out, inn, code)
     if n <= 0:
-        return None, 0, 0
-    ws = L._torch().empty(n, dtype=L._torch().uint8, device=device)
+        return None, None, 0
+    ws = a.new_empty(n, dtype=L._torch().uint8)
     return ws, ws.data_ptr(), n
 
 
 def _product(name, op, x, w, out, out_dtype, dtype, what):
-    if not isinstance(w, QuantizedTensor) or w.kind not in _W4:
+    if not isinstance(w, QuantizedTensor) or w.kind not in _BLOCK:
         raise L.OdysseyError(f"{name} takes a weight of the 4-bit kinds", L.ERR_ARG)
     r = _Rows(x, dtype, what)
     features, numel = r.cols, w.original_numel
@@ -172,34 +184,34 @@ def _product(name, op, x, w, out, out_dtype, dtype, what):
         raise L.OdysseyError(f"{name}: a weight of {numel} elements has no rows of {features}" if op == L.LINEAR_FORWARD
                              else f"{name}: a weight of {numel} elements does not have {features} rows", L.ERR_SHAPE)
     nout, nin = (other, features) if op == L.LINEAR_FORWARD else (features, other)
-    if L.numel(w.data) != L.quant_bytes(w.kind, numel):
-        raise L.OdysseyError(f"quantised buffer has {L.numel(w.data)} bytes, expected "
-                             f"{L.quant_bytes(w.kind, numel)}", L.ERR_SHAPE)
+    block, size = _BLOCK[w.kind]
+    need = (numel + block - 1) // block * size
+    data = w.data
+    if L.numel(data) != need:
+        raise L.OdysseyError(f"quantised buffer has {L.numel(data)} bytes, expected {need}", L.ERR_SHAPE)
     code = r.code if out_dtype is None else _code(out_dtype)
     y = _out(r, out, r.lead + (other,), code, "out")
     lib = L.lib()
-    if r.cuda:
-        _same_place(r, w.data)
-        data = w.data if w.data.is_contiguous() else w.data.contiguous()
-        ts, alpha = None, 1.0
-        if w.kind == L.Q_NVFP4_TENSOR:
-            if L.is_torch(w.tensor_scale):  # a device float: read by the kernel, no synchronisation
-                _same_place(r, w.tensor_scale)
-                if w.tensor_scale.numel() != 1 or w.tensor_scale.dtype != L._torch().float32:
-                    raise L.OdysseyError("the tensor scale must be one float32", L.ERR_DTYPE)
-                ts = w.tensor_scale.data_ptr()
-            else:
-                alpha = w.tensor_scale
-        fn = lib.ody_fp4_linear_on_stream if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad_on_stream
-        with _On(r.a.device) as st:
-            ws, wp, wn = _workspace(op, r.rows, nout, nin, r.code, r.a.device)
-            L.check(fn(w.kind, data.data_ptr(), ts, alpha, nout, nin, r.ptr, r.code, r.rows, r.ld, y.data_ptr(), code,
-                       other, wp, wn, st))
+    _same_place(r, data)
+    if not r.cuda:
+        fn = lib.ody_fp4_linear if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad
+        L.check(fn(w.kind, L.ptr(L.contiguous(data)), float(w.tensor_scale), nout, nin, r.ptr, r.code, r.rows, L.ptr(y),
+                   code))
         return y
-    _same_place(r, w.data)
-    fn = lib.ody_fp4_linear if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad
-    L.check(fn(w.kind, L.ptr(L.contiguous(w.data)), float(w.tensor_scale), nout, nin, r.ptr, r.code, r.rows, L.ptr(y),
-               code))
+    data = _flat(data)
+    ts, alpha = None, 1.0
+    if w.kind == L.Q_NVFP4_TENSOR:
+        if L.is_torch(w.tensor_scale):  # a device float: read by the kernel, no synchronisation
+            _same_place(r, w.tensor_scale)
+            if w.tensor_scale.numel() != 1 or w.tensor_scale.dtype != L._torch().float32:
+                raise L.OdysseyError("the tensor scale must be one float32", L.ERR_DTYPE)
+            ts = w.tensor_scale.data_ptr()
+        else:
+            alpha = w.tensor_scale
+    fn = lib.ody_fp4_linear_on_stream if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad_on_stream
+    ws, at, n = _workspace(r.a, op, r.rows, nout, nin, r.code)
+    _enqueue(r.a.device, lambda st: fn(w.kind, data.data_ptr(), ts, alpha, nout, nin, r.ptr, r.code, r.rows, r.ld,
+                                       y.data_ptr(), code, other, at, n, st))
     return y
 
 
@@ -218,23 +230,22 @@ def fp4_linear_dgrad(dy, w, out=None, out_dtype=None, dtype=None):
 def save_activation8(x, format="e4m3", dtype=None):
     """x[..., cols] in 8 bits ('e4m3' or 'e5m2') with a power of two per 32
     columns, the least that keeps the group's largest finite element in range."""
-    if format not in FORMATS8:
+    fmt = FORMATS8.get(format)
+    if fmt is None:
         raise L.OdysseyError(f"unknown 8-bit activation format {format!r}", L.ERR_ARG)
     r = _Rows(x, dtype, "x")
     g = (r.cols + 31) // 32
     if L.is_torch(r.a):
-        t = L._torch()
-        # one allocation: the codes' rows, then the scales
-        buf = t.empty(r.rows * g * 33, dtype=t.uint8, device=r.a.device)
-        codes, scales = buf[:r.rows * g * 32].view(r.rows, g * 32), buf[r.rows * g * 32:].view(r.rows, g)
+        u8 = L._torch().uint8
+        codes, scales = r.a.new_empty((r.rows, g * 32), dtype=u8), r.a.new_empty((r.rows, g), dtype=u8)
     else:
         codes, scales = np.empty((r.rows, g * 32), np.uint8), np.empty((r.rows, g), np.uint8)
+    lib = L.lib()
     if r.cuda:
-        with _On(r.a.device) as st:
-            L.check(L.lib().ody_act8_save_on_stream(FORMATS8[format], r.ptr, r.code, r.rows, r.cols, r.ld,
-                                                    codes.data_ptr(), scales.data_ptr(), st))
+        _enqueue(r.a.device, lambda st: lib.ody_act8_save_on_stream(fmt, r.ptr, r.code, r.rows, r.cols, r.ld,
+                                                                    codes.data_ptr(), scales.data_ptr(), st))
     else:
-        L.check(L.lib().ody_act8_save(FORMATS8[format], r.ptr, r.code, r.rows, r.cols, L.ptr(codes), L.ptr(scales)))
+        L.check(lib.ody_act8_save(fmt, r.ptr, r.code, r.rows, r.cols, L.ptr(codes), L.ptr(scales)))
     return Activation8(codes, scales, r.rows, r.cols, format, r.lead + (r.cols,), _NAMES[r.code])
 
 
@@ -247,20 +258,13 @@ def load_activation8(a, dtype=None, out=None):
     r = _Place(codes)
     _same_place(r, scales)
     y = _out(r, out, shape, code, "out")
-    fn, c, s = L.lib(), L.ptr(codes), L.ptr(scales)
+    lib, fmt = L.lib(), FORMATS8[a.format]
     if r.cuda:
-        with _On(codes.device) as st:
-            L.check(fn.ody_act8_load_on_stream(FORMATS8[a.format], c, s, a.rows, a.cols, y.data_ptr(), code, a.cols, st))
+        _enqueue(codes.device, lambda st: lib.ody_act8_load_on_stream(fmt, codes.data_ptr(), scales.data_ptr(), a.rows,
+                                                                      a.cols, y.data_ptr(), code, a.cols, st))
     else:
-        L.check(fn.ody_act8_load(FORMATS8[a.format], c, s, a.rows, a.cols, L.ptr(y), code))
+        L.check(lib.ody_act8_load(fmt, L.ptr(codes), L.ptr(scales), a.rows, a.cols, L.ptr(y), code))
     return y
-
-
-class _Place:
-    """Where a buffer lies (what _same_place and _out ask of _Rows)."""
-
-    def __init__(self, a):
-        self.a, self.cuda = a, L.is_torch(a) and a.is_cuda
 
 
 def linear_wgrad8(dy, a, add=None, alpha=1.0, out=None, out_dtype=None, dtype=None):
@@ -279,17 +283,18 @@ def linear_wgrad8(dy, a, add=None, alpha=1.0, out=None, out_dtype=None, dtype=No
         like = out if out is not None else add
         code = r.code if like is None else \
             (L.BF16 if not L.is_torch(like) and like.dtype == np.uint16 else L.dtype_code(like))
-    y = _out(r, out, (r.cols, a.cols), code, "out")
+    shape = (r.cols, a.cols)
+    y = _out(r, out, shape, code, "out")
     if add is not None:
-        add = _out(r, add, (r.cols, a.cols), code, "add")
+        add = _out(r, add, shape, code, "add")
     codes, scales = L.contiguous(a.codes), L.contiguous(a.scales)
     fmt, lib = FORMATS8[a.format], L.lib()
     if r.cuda:
-        with _On(r.a.device) as st:
-            ws, wp, wn = _workspace(L.LINEAR_WGRAD, r.rows, r.cols, a.cols, r.code, r.a.device)
-            L.check(lib.ody_linear_wgrad8_on_stream(fmt, codes.data_ptr(), scales.data_ptr(), a.rows, a.cols, r.ptr,
-                                                    r.code, r.cols, r.ld, alpha, None if add is None else add.data_ptr(),
-                                                    y.data_ptr(), code, wp, wn, st))
+        ws, at, n = _workspace(r.a, L.LINEAR_WGRAD, r.rows, r.cols, a.cols, r.code)
+        plus = None if add is None else add.data_ptr()
+        _enqueue(r.a.device, lambda st: lib.ody_linear_wgrad8_on_stream(
+            fmt, codes.data_ptr(), scales.data_ptr(), a.rows, a.cols, r.ptr, r.code, r.cols, r.ld, alpha, plus,
+            y.data_ptr(), code, at, n, st))
     else:
         L.check(lib.ody_linear_wgrad8(fmt, L.ptr(codes), L.ptr(scales), a.rows, a.cols, r.ptr, r.code, r.cols,
                                       C.c_float(alpha), None if add is None else L.ptr(add), L.ptr(y), code))
@@ -301,5 +306,5 @@ def linear_status(device=None):
     wait inside a linear kernel ran out there since the last query (the CUDA
     calls above do not wait, so they cannot say so themselves)."""
     t = L._torch()
-    with _On(t.device("cuda", t.cuda.current_device() if device is None else t.device(device).index)) as st:
-        L.check(L.lib().ody_linear_status(st))
+    index = None if device is None else t.device(device).index
+    _enqueue(t.device("cuda", t.cuda.current_device() if index is None else index), L.lib().ody_linear_status)
