@@ -79,6 +79,20 @@ def test_product_block_tails(ody, inn):
             forward_case(ody, inn, kind, 70, 51, inn, "bfloat16", dgrad=dgrad)
 
 
+# past the one-launch kernels: whole and ragged tiles of the tcgen05 kernel,
+# tiles shared by steps, widths of whole blocks and others
+LARGE = [(700, 1100, 1030), (2048, 512, 1024), (300, 2500, 1999), (1025, 769, 1568), (64, 4100, 4096), (257, 3000, 4112),
+         (4000, 1300, 264)]
+
+
+@pytest.mark.parametrize("rows,out,inn", LARGE)
+@pytest.mark.parametrize("dgrad", [False, True], ids=["forward", "dgrad"])
+def test_large_products(ody, rows, out, inn, dgrad):
+    for i, (kind, dtype, out_dtype) in enumerate((("nvfp4", "bfloat16", None), ("mxfp4", "float32", None),
+                                                  ("mxfp4_ocp", "float16", "float32"), ("nvfp4_tensor", "bfloat16", "float16"))):
+        forward_case(ody, rows + i, kind, rows, out, inn, dtype, out_dtype, dgrad, pad=(0, 0, 8, 9)[i])
+
+
 @pytest.mark.parametrize("out_dtype", DTYPES)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_product_types_and_pitches(ody, dtype, out_dtype):
@@ -158,7 +172,7 @@ def test_float32_rows_use_all_their_bits(ody):
         blocks[e // 16, (e % 16) // 2] = 0x20 if e % 2 == 0 else 0x02
     blocks[:, -1] = 56  # 1.0
     w = ody.QuantizedTensor(dev(blocks.reshape(-1)), R.NVFP4, inn * inn)
-    for rows in (1, 8, 200):
+    for rows in (1, 8, 200, 12000):
         x = rng.standard_normal((rows, inn)).astype(np.float32) * np.exp2(rng.integers(-90, 100, (rows, 1))).astype(np.float32)
         x[:, 3] = np.float32(1.0) + np.float32(2.0 ** -23)
         x[:, 4] = np.finfo(np.float32).max
@@ -172,11 +186,11 @@ def test_float32_rows_use_all_their_bits(ody):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows", [1, 6, 40, 200])
-def test_non_finite_inputs_stay_in_their_row(ody, rows, dtype):
+@pytest.mark.parametrize("rows,inn", [(1, 272), (6, 272), (40, 272), (200, 272), (2000, 4112)])
+def test_non_finite_inputs_stay_in_their_row(ody, rows, inn, dtype):
     rng = np.random.default_rng(rows)
-    w, w64 = make_w(ody, rng, "nvfp4", 48, 272)
-    x = rng.standard_normal((rows, 272)).astype(np.float32)
+    w, w64 = make_w(ody, rng, "nvfp4", 48, inn)
+    x = rng.standard_normal((rows, inn)).astype(np.float32)
     bad = rows // 2
     for value in (np.inf, -np.inf, np.nan):
         x[bad, 5] = value
@@ -191,7 +205,7 @@ def test_non_finite_inputs_stay_in_their_row(ody, rows, dtype):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("rows", [1, 100])
+@pytest.mark.parametrize("rows", [1, 100, 9000])
 def test_non_finite_block_stays_in_its_results(ody, kind, rows):
     k = R.W4_KINDS[kind]
     be, sb = R.block(k)
@@ -363,6 +377,14 @@ def test_wgrad_shapes(ody, rows, out, inn):
             wgrad_case(ody, rows, rows, out, inn, dtype, dtype, fmt, add=True, alpha=0.25)
 
 
+@pytest.mark.parametrize("rows,out,inn", [(1500, 1100, 1030), (20000, 64, 64), (700, 2048, 1000), (3001, 520, 1313),
+                                          (4096, 1024, 512)])
+def test_large_wgrads(ody, rows, out, inn):
+    for i, (fmt, dtype, out_dtype) in enumerate((("e4m3", "bfloat16", "bfloat16"), ("e5m2", "float16", "float32"),
+                                                 ("e4m3", "float32", "float32"), ("e4m3", "bfloat16", "float16"))):
+        wgrad_case(ody, rows + i, rows, out, inn, dtype, out_dtype, fmt, add=i % 2 == 1, alpha=0.5, pad=(0, 0, 0, 9)[i])
+
+
 @pytest.mark.parametrize("out_dtype", DTYPES)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_wgrad_types_and_pitches(ody, dtype, out_dtype):
@@ -430,7 +452,7 @@ def test_gradients_against_differences(ody):
 # ---- streams, graphs, repeats, neighbours -----------------------------------
 def test_same_call_same_bits(ody):
     rng = np.random.default_rng(6)
-    for rows, out, inn in ((1, 512, 1024), (8, 500, 528), (300, 256, 2048), (2000, 96, 160)):
+    for rows, out, inn in ((1, 512, 1024), (8, 500, 528), (300, 256, 2048), (2000, 96, 160), (1111, 1300, 1040)):
         w, _ = make_w(ody, rng, "nvfp4", out, inn)
         x = dev(rng.standard_normal((rows, inn)).astype(np.float32))
         dy = dev(rng.standard_normal((rows, out)).astype(np.float32), "bfloat16")
@@ -447,7 +469,7 @@ def test_captured_and_replayed_on_side_streams(ody):
     with new inputs, give the bits of eager calls."""
     rng = np.random.default_rng(7)
     sets = []
-    for rows, out, inn in ((200, 384, 640), (3, 257, 1040)):
+    for rows, out, inn in ((900, 1100, 1040), (200, 384, 640), (3, 257, 1040)):
         w, _ = make_w(ody, rng, "mxfp4", out, inn)
         x = dev(rng.standard_normal((rows, inn)).astype(np.float32), "bfloat16")
         dy = dev(rng.standard_normal((rows, out)).astype(np.float32), "bfloat16")
@@ -483,8 +505,8 @@ def test_captured_and_replayed_on_side_streams(ody):
 
 def test_overlapping_calls_on_two_streams(ody):
     rng = np.random.default_rng(17)
-    w, _ = make_w(ody, rng, "nvfp4", 512, 768)
-    xs = [dev(rng.standard_normal((150, 768)).astype(np.float32)) for _ in range(2)]
+    w, _ = make_w(ody, rng, "nvfp4", 1500, 768)
+    xs = [dev(rng.standard_normal((950, 768)).astype(np.float32)) for _ in range(2)]
     want = [ody.fp4_linear(x, w) for x in xs]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in xs]
@@ -498,14 +520,13 @@ def test_overlapping_calls_on_two_streams(ody):
         assert all(torch.equal(g, want[i]) for g in got[i])
 
 
-@pytest.mark.parametrize("rows", [1, 5, 70, 300])
-def test_pitched_outputs_leave_their_neighbours(ody, rows):
+@pytest.mark.parametrize("rows,out,inn", [(1, 72, 144), (5, 72, 144), (70, 72, 144), (300, 72, 144), (500, 1503, 1552)])
+def test_pitched_outputs_leave_their_neighbours(ody, rows, out, inn):
     """The stream forms write rows x columns of the output and nothing else,
     with float16, bfloat16 and float32 results at odd pitches."""
     from odyssey_b200 import _lib as L
     lib = L.lib()
     rng = np.random.default_rng(rows)
-    out, inn = 72, 144
     w, w64 = make_w(ody, rng, "mxfp4", out, inn)
     st = torch.cuda.current_stream().cuda_stream
     for op, cols, width in ((L.LINEAR_FORWARD, inn, out), (L.LINEAR_DGRAD, out, inn)):
