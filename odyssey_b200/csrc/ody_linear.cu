@@ -32,8 +32,8 @@ namespace ody {
 // An operand's tile lies in shared memory as it does in memory, rows of 64
 // elements at 144 bytes (nine 16-byte words: ldmatrix reads eight rows
 // without a bank conflict); where those rows are the reduction's the
-// fragments are read transposed.  Every 512 products the sums are added in
-// float32 with rounding, as in the tcgen05 kernel.
+// fragments are read transposed.  Every 32 mma the sums are added in float32
+// with rounding, as in the tcgen05 kernel.
 // ---------------------------------------------------------------------------
 constexpr int kMT = 64, kMPitch = 144, kMTile = kMT * kMPitch, kMSumPitch = kMT + 4;
 
@@ -133,12 +133,10 @@ struct EightQ {
   __device__ __forceinline__ void store(uint8_t* d) const {
     uint32_t o[4];
     if constexpr (OP == LIN_WGRAD) {
+      float v[8];
+      a8_values8<KIND>(make_uint2(code[0], code[1]), scale, v);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint32_t two = code[i >> 1] >> (16 * (i & 1));
-        o[i] = __byte_perm(__float_as_uint(a8_value<KIND>(two & 255u, scale)),
-                           __float_as_uint(a8_value<KIND>((two >> 8) & 255u, scale)), 0x7632);
-      }
+      for (int i = 0; i < 4; i++) o[i] = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
     } else {
       w4_raw8<KIND>(code[0], o);
       const uint32_t f0 = w4_scale_bf16x2<KIND>(scale & 255u), f1 = w4_scale_bf16x2<KIND>(scale >> 8 & 255u);
@@ -168,7 +166,7 @@ __device__ __forceinline__ void ldmatrix4(uint32_t at, uint32_t r[4]) {
 
 template <int OP, int KIND, int DT>
 __global__ void __launch_bounds__(256) medium_kernel(const LinearArgs p) {
-  constexpr int P = bf16_parts(DT), STAGE = (P + 1) * kMTile;
+  constexpr int P = bf16_parts(DT), STAGE = (P + 1) * kMTile, KEEP = 8 / P;  // steps of 4 P mma in one sum
   constexpr bool AR = OP != LIN_WGRAD, BR = OP == LIN_FORWARD;  // the contiguous axis is the reduction's
   extern __shared__ __align__(16) uint8_t medium_sm[];
   const int64_t M = OP == LIN_WGRAD ? p.out : p.rows, N = OP == LIN_FORWARD ? p.out : p.in;
@@ -239,7 +237,7 @@ __global__ void __launch_bounds__(256) medium_kernel(const LinearArgs p) {
         for (int j = 0; j < 4; j++) mma16816(part[j], x[0], x[1], x[2], x[3], y[j >> 1][2 * (j & 1)], y[j >> 1][2 * (j & 1) + 1]);
       }
     }
-    if (((s - s0) & 7) == 7 || s + 1 == s1) {
+    if ((s - s0) % KEEP == KEEP - 1 || s + 1 == s1) {
 #pragma unroll
       for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -387,10 +385,10 @@ template <int FMT>
 struct A8 {
   static constexpr int TOP = FMT == A8_E4M3 ? 8 : 15;
   static constexpr int XMIN = FMT == A8_E4M3 ? -117 : -110, XMAX = FMT == A8_E4M3 ? 119 : 112;
-  static __device__ __forceinline__ int exponent(float amax) {
-    const uint32_t b = __float_as_uint(amax);
-    const int x = (int)(b >> 23) - 127 - TOP + ((b & 0x7fffffu) > 0x600000u);
-    return x < XMIN ? XMIN : (x > XMAX ? XMAX : x);  // subnormal amax: below XMIN anyway
+  // the power for a finite amax (its bits); subnormal ones are below XMIN anyway
+  static __device__ __forceinline__ int exponent(uint32_t amax) {
+    const int x = (int)(amax >> 23) - 127 - TOP + ((amax & 0x7fffffu) > 0x600000u);
+    return min(max(x, XMIN), XMAX);
   }
   static __device__ __forceinline__ uint32_t encode(float x, float inv) {
     const uint32_t sign = (__float_as_uint(x) >> 24) & 0x80u;
@@ -398,83 +396,161 @@ struct A8 {
     const float v = __fmul_rn(x, inv);
     return FMT == A8_E4M3 ? f32_to_e4m3(v) : f32_to_e5m2(v);
   }
+  // two finite values; the first in the low byte
+  static __device__ __forceinline__ uint32_t encode2(float x, float y, float inv) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(x, inv), __fmul_rn(y, inv)), __NV_SATFINITE,
+                                    FMT == A8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+  }
 };
 
-// Four lanes share a group, eight elements each: two 16-byte loads of float32
-// or one of 16-bit elements where the row's alignment allows it.
+// Both directions move 1 + 1/32 bytes a value on one side and the value on
+// the other, so they are bound by memory; a thread has four runs of eight
+// values under way, and what it does to them is counted: the largest
+// magnitude of 16-bit values is found on their bits, two at a time, values
+// are converted in pairs, and only a warp that meets a NaN or infinity looks
+// at single elements (8192 x 4096 in bfloat16: element by element 37 us).
+constexpr int kRuns = 4;
+
+// eight elements: the bits as they lie, their largest magnitude (as the bits
+// of a float32), and as float32
+template <int DT>
+struct Run8 {
+  uint4 raw[DT == DT_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* x, int64_t at, int n, bool wide) {
+    if (wide && n >= 8) {
+      const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(x) + at * (DT == DT_F32 ? 4 : 2));
+#pragma unroll
+      for (int i = 0; i < (DT == DT_F32 ? 2 : 1); i++) raw[i] = __ldcs(s + i);
+    } else {
+      uint32_t w[DT == DT_F32 ? 8 : 4] = {};
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (i < n) {
+          if constexpr (DT == DT_F32)
+            w[i] = __ldg(reinterpret_cast<const uint32_t*>(x) + at + i);
+          else
+            w[i >> 1] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(x) + at + i) << (16 * (i & 1));
+        }
+#pragma unroll
+      for (int i = 0; i < (DT == DT_F32 ? 2 : 1); i++) raw[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+  }
+  __device__ __forceinline__ uint32_t word(int i) const {
+    const uint4& u = raw[DT == DT_F32 ? i >> 2 : 0];
+    const int k = i & 3;
+    return k == 0 ? u.x : (k == 1 ? u.y : (k == 2 ? u.z : u.w));
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if (DT == DT_F32) return __uint_as_float(word(i));
+    const uint32_t w = word(i >> 1);
+    if (DT == DT_BF16) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    return f16_bits_to_f32((uint16_t)(i & 1 ? w >> 16 : w));
+  }
+  // a NaN or infinity: 0x7f800000 or more
+  __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = 0;
+    if constexpr (DT == DT_F32) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) m = max(m, word(i) & 0x7fffffffu);
+      return m;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) m = __vmaxu2(m, word(i) & 0x7fff7fffu);
+      m = max(m >> 16, m & 0xffffu);
+      return DT == DT_BF16 ? m << 16 : __float_as_uint(f16_bits_to_f32((uint16_t)m));
+    }
+  }
+};
+
+// the row and first column of eight values; flat: rows lie one behind the
+// other in whole groups, as the codes do
+struct Spot8 {
+  int64_t row, col;
+};
+__device__ __forceinline__ Spot8 spot8(int64_t t, int64_t groups, bool flat) {
+  if (flat) return {0, t * 8};
+  const int64_t g = t >> 2, row = (uint64_t)g >> 32 ? g / groups : (uint32_t)g / (uint32_t)groups;
+  return {row, (g - row * groups) * kA8Group + (t & 3) * 8};
+}
+
+// Four lanes share a group, eight elements each.
 template <int FMT, int DT>
 __global__ void __launch_bounds__(256) act8_save_kernel(const void* x, int64_t rows, int64_t cols, int64_t ldx,
-                                                        uint8_t* codes, uint8_t* scales, int wide) {
-  const int64_t groups = (cols + kA8Group - 1) / kA8Group;
-  const int64_t total = rows * groups * 4;
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < (total + 31) / 32 * 32; t += stride) {
-    float v[8] = {};
-    const bool on = t < total;
-    const int64_t g = t >> 2, row = on ? g / groups : 0;
-    const int64_t c0 = (g - row * groups) * kA8Group + (t & 3) * 8;
-    if (on) {
-      const int64_t at = row * ldx + c0;
-      if (wide && c0 + 8 <= cols) {
-        if (DT == DT_F32) {
-          const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + at);
-          const float4 a = __ldcs(s), b = __ldcs(s + 1);
-          v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-          const uint4 u = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + at));
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                                                        uint8_t* codes, uint8_t* scales, int wide, int flat) {
+  const int64_t groups = (cols + kA8Group - 1) / kA8Group, total = rows * groups * 4;
+  const int64_t t0 = (int64_t)blockIdx.x * 256 * kRuns + threadIdx.x;
+  Run8<DT> v[kRuns];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            v[2 * i] = DT == DT_F16 ? f16_bits_to_f32(w[i] & 0xffff) : bf16_bits_to_f32(w[i] & 0xffff);
-            v[2 * i + 1] = DT == DT_F16 ? f16_bits_to_f32(w[i] >> 16) : bf16_bits_to_f32(w[i] >> 16);
-          }
-        }
-      } else {
+  for (int r = 0; r < kRuns; r++) {
+    const int64_t t = t0 + r * 256;
+    const Spot8 s = spot8(t, groups, flat);
+    v[r].load(x, s.row * ldx + s.col, t < total ? (flat ? 8 : (int)min((int64_t)8, cols - s.col)) : 0, wide);
+  }
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-          if (c0 + i < cols) v[i] = load_elem(x, DT, at + i);
+  for (int r = 0; r < kRuns; r++) {
+    const int64_t t = t0 + r * 256;
+    uint32_t amax = v[r].amax();
+    const bool odd = __any_sync(0xffffffffu, amax >= 0x7f800000u);
+    if (odd) {  // of the finite elements only
+      amax = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const uint32_t m = __float_as_uint(v[r].at(i)) & 0x7fffffffu;
+        if (m < 0x7f800000u) amax = max(amax, m);
       }
     }
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float a = fabsf(v[i]);
-      amax = a < __uint_as_float(0x7f800000u) ? fmaxf(amax, a) : amax;  // finite elements only
-    }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    if (!on) continue;
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const int ex = A8<FMT>::exponent(amax);
     const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);
-    uint32_t lo = 0, hi = 0;
+    uint32_t lo, hi;
+    if (odd) {
+      lo = hi = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      lo |= A8<FMT>::encode(v[i], inv) << (8 * i);
-      hi |= A8<FMT>::encode(v[4 + i], inv) << (8 * i);
+      for (int i = 0; i < 4; i++) {
+        lo |= A8<FMT>::encode(v[r].at(i), inv) << (8 * i);
+        hi |= A8<FMT>::encode(v[r].at(4 + i), inv) << (8 * i);
+      }
+    } else {
+      lo = A8<FMT>::encode2(v[r].at(0), v[r].at(1), inv) | A8<FMT>::encode2(v[r].at(2), v[r].at(3), inv) << 16;
+      hi = A8<FMT>::encode2(v[r].at(4), v[r].at(5), inv) | A8<FMT>::encode2(v[r].at(6), v[r].at(7), inv) << 16;
     }
+    // eight groups of the warp: their scales in two words
+    uint32_t sb = (uint32_t)(ex + 127);
+    sb |= __shfl_down_sync(0xffffffffu, sb, 4) << 8;
+    sb |= __shfl_down_sync(0xffffffffu, sb, 8) << 16;
+    if (t >= total) continue;
     __stcs(reinterpret_cast<uint2*>(codes) + t, make_uint2(lo, hi));
-    if ((t & 3) == 0) scales[g] = (uint8_t)(ex + 127);
+    const int64_t g = t >> 2;
+    if ((threadIdx.x & 15) == 0 && t + 16 <= total && (reinterpret_cast<uintptr_t>(scales) & 3u) == 0)
+      reinterpret_cast<uint32_t*>(scales)[g >> 2] = sb;
+    else if ((threadIdx.x & 3) == 0 && ((t & ~(int64_t)15) + 16 > total || (reinterpret_cast<uintptr_t>(scales) & 3u)))
+      scales[g] = (uint8_t)sb;
   }
 }
 
 template <int FMT, int DT>
 __global__ void __launch_bounds__(256) act8_load_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows,
-                                                        int64_t cols, void* out, int64_t ldo, int wide) {
-  const int64_t groups = (cols + kA8Group - 1) / kA8Group;
-  const int64_t total = rows * groups * 4;
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < total; t += stride) {
-    const int64_t g = t >> 2, row = g / groups;
-    const int64_t c0 = (g - row * groups) * kA8Group + (t & 3) * 8;
-    if (c0 >= cols) continue;
-    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(codes) + t);
-    const uint32_t sb = scales[g];
-    float v[8];
+                                                        int64_t cols, void* out, int64_t ldo, int wide, int flat) {
+  const int64_t groups = (cols + kA8Group - 1) / kA8Group, total = rows * groups * 4;
+  const int64_t t0 = (int64_t)blockIdx.x * 256 * kRuns + threadIdx.x;
+  uint2 c[kRuns];
+  uint32_t sb[kRuns];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      v[i] = a8_value<FMT>((w.x >> (8 * i)) & 255u, sb);
-      v[4 + i] = a8_value<FMT>((w.y >> (8 * i)) & 255u, sb);
-    }
+  for (int r = 0; r < kRuns; r++) {
+    const int64_t t = min(t0 + r * 256, total - 1);
+    c[r] = __ldcs(reinterpret_cast<const uint2*>(codes) + t);
+    sb[r] = __ldg(scales + (t >> 2));
+  }
+#pragma unroll
+  for (int r = 0; r < kRuns; r++) {
+    const int64_t t = t0 + r * 256;
+    if (t >= total) return;
+    const Spot8 s = spot8(t, groups, flat);
+    const int n = flat ? 8 : (int)min((int64_t)8, cols - s.col);
+    if (n <= 0) continue;
+    float v[8];
+    a8_values8<FMT>(c[r], sb[r], v);
     if (DT == DT_F16) {
       // a finite value that rounded past float16's largest stays finite (it
       // came from a finite element); an infinity stays one
@@ -482,8 +558,8 @@ __global__ void __launch_bounds__(256) act8_load_kernel(const uint8_t* codes, co
       for (int i = 0; i < 8; i++)
         if (fabsf(v[i]) < __uint_as_float(0x7f800000u)) v[i] = fminf(fmaxf(v[i], -65504.0f), 65504.0f);
     }
-    const int64_t at = row * ldo + c0;
-    if (wide && c0 + 8 <= cols) {
+    const int64_t at = s.row * ldo + s.col;
+    if (wide && n == 8) {
       if (DT == DT_F32) {
         float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
         __stcs(d, make_float4(v[0], v[1], v[2], v[3]));
@@ -491,23 +567,21 @@ __global__ void __launch_bounds__(256) act8_load_kernel(const uint8_t* codes, co
       } else {
         uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4; i++)  // bfloat16 holds the values exactly
           u[i] = DT == DT_F16 ? f32_to_f16_bits(v[2 * i]) | (uint32_t)f32_to_f16_bits(v[2 * i + 1]) << 16
-                              : f32_to_bf16_bits(v[2 * i]) | (uint32_t)f32_to_bf16_bits(v[2 * i + 1]) << 16;
+                              : __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
         __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + at), make_uint4(u[0], u[1], u[2], u[3]));
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        if (c0 + i < cols) store_elem(out, DT, at + i, v[i]);
+        if (i < n) store_elem(out, DT, at + i, v[i]);
     }
   }
 }
 
-static int act8_grid(int64_t rows, int64_t cols) {
-  const int64_t want = (rows * ((cols + kA8Group - 1) / kA8Group) * 4 + 255) / 256;
-  const int64_t cap = (int64_t)lin_sms() * 32;
-  return (int)(want < cap ? want : cap);
+static unsigned act8_grid(int64_t rows, int64_t cols) {
+  return (unsigned)((rows * ((cols + kA8Group - 1) / kA8Group) * 4 + 256 * kRuns - 1) / (256 * kRuns));
 }
 
 // whether 16-byte accesses at multiples of eight columns are aligned
@@ -518,9 +592,10 @@ static int wide_rows(const void* p, int dtype, int64_t ld) {
 
 cudaError_t launch_act8_save(int fmt, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* codes,
                              uint8_t* scales, cudaStream_t st) {
-  const int grid = act8_grid(rows, cols), w = wide_rows(x, dtype, ldx);
+  const unsigned grid = act8_grid(rows, cols);
+  const int w = wide_rows(x, dtype, ldx), flat = ldx == cols && cols % kA8Group == 0;
 #define ODY_S(F, D) \
-  if (fmt == F && dtype == D) act8_save_kernel<F, D><<<grid, 256, 0, st>>>(x, rows, cols, ldx, codes, scales, w);
+  if (fmt == F && dtype == D) act8_save_kernel<F, D><<<grid, 256, 0, st>>>(x, rows, cols, ldx, codes, scales, w, flat);
   ODY_S(A8_E4M3, DT_F32) ODY_S(A8_E4M3, DT_F16) ODY_S(A8_E4M3, DT_BF16)
   ODY_S(A8_E5M2, DT_F32) ODY_S(A8_E5M2, DT_F16) ODY_S(A8_E5M2, DT_BF16)
 #undef ODY_S
@@ -529,9 +604,10 @@ cudaError_t launch_act8_save(int fmt, const void* x, int dtype, int64_t rows, in
 
 cudaError_t launch_act8_load(int fmt, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* out,
                              int dtype, int64_t ldo, cudaStream_t st) {
-  const int grid = act8_grid(rows, cols), w = wide_rows(out, dtype, ldo);
+  const unsigned grid = act8_grid(rows, cols);
+  const int w = wide_rows(out, dtype, ldo), flat = ldo == cols && cols % kA8Group == 0;
 #define ODY_L(F, D) \
-  if (fmt == F && dtype == D) act8_load_kernel<F, D><<<grid, 256, 0, st>>>(codes, scales, rows, cols, out, ldo, w);
+  if (fmt == F && dtype == D) act8_load_kernel<F, D><<<grid, 256, 0, st>>>(codes, scales, rows, cols, out, ldo, w, flat);
   ODY_L(A8_E4M3, DT_F32) ODY_L(A8_E4M3, DT_F16) ODY_L(A8_E4M3, DT_BF16)
   ODY_L(A8_E5M2, DT_F32) ODY_L(A8_E5M2, DT_F16) ODY_L(A8_E5M2, DT_BF16)
 #undef ODY_L

@@ -75,10 +75,16 @@ __device__ __forceinline__ void w4_raw8(uint32_t w, uint32_t o[4]) {
 }
 constexpr uint32_t kTwo126 = 0x7e807e80u;  // 2^126 as a bfloat16 pair
 
+// the values of eight codes
 template <int FMT>
-__device__ __forceinline__ float a8_value(uint32_t code, uint32_t scale_byte) {
-  const float v = FMT == A8_E4M3 ? e4m3_to_f32((uint8_t)code) : e5m2_to_f32((uint8_t)code);
-  return __fmul_rn(v, __uint_as_float(scale_byte << 23));
+__device__ __forceinline__ void a8_values8(uint2 c, uint32_t scale_byte, float v[8]) {
+  const float f = __uint_as_float(scale_byte << 23);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t two = (i < 2 ? c.x : c.y) >> (16 * (i & 1));
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, FMT == A8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+    v[2 * i] = __fmul_rn(f16_bits_to_f32(h.x), f), v[2 * i + 1] = __fmul_rn(f16_bits_to_f32(h.y), f);
+  }
 }
 
 __device__ __forceinline__ float load_elem(const void* p, int dt, int64_t i) {

@@ -86,19 +86,26 @@ __global__ void __launch_bounds__(256) unpack_a8_kernel(const uint8_t* __restric
                                                         const uint8_t* __restrict__ scales, int64_t n8,
                                                         uint16_t* __restrict__ out) {
   let_next_start();
+  const int64_t t0 = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+  uint2 cs[4];
+  uint32_t sbs[4];
 #pragma unroll
   for (int h = 0; h < 4; h++) {
-    const int64_t t = (int64_t)blockIdx.x * 1024 + h * 256 + threadIdx.x;
-    if (t >= n8) return;
-    const uint2 c = __ldcs(reinterpret_cast<const uint2*>(codes) + t);
-    const uint32_t sb = scales[t >> 2];
-    uint32_t o[4];
+    const int64_t t = min(t0 + h * 256, n8 - 1);
+    cs[h] = __ldcs(reinterpret_cast<const uint2*>(codes) + t);
+    sbs[h] = __ldg(scales + (t >> 2));
+  }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const uint32_t two = (i < 2 ? c.x : c.y) >> (16 * (i & 1));
-      o[i] = (__float_as_uint(a8_value<FMT>(two & 255u, sb)) >> 16) |
-             (__float_as_uint(a8_value<FMT>((two >> 8) & 255u, sb)) & 0xffff0000u);
-    }
+  for (int h = 0; h < 4; h++) {
+    const int64_t t = t0 + h * 256;
+    if (t >= n8) return;
+    const uint2 c = cs[h];
+    const uint32_t sb = sbs[h];
+    float v[8];
+    uint32_t o[4];
+    a8_values8<FMT>(c, sb, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
     reinterpret_cast<uint4*>(out)[t] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
