@@ -60,33 +60,36 @@ struct Ring {
 
   // Columns k0.. of rows r0.. into a stage; neighbouring lanes copy
   // neighbouring words of a row (two lanes to a row, each with every other
-  // word, halved the rate).  Words that lie wholly inside the weight's bytes
-  // are copied asynchronously; the first and the last bytes of the weight,
-  // which only its first and last tiles hold, one by one.
+  // word, halved the rate).  What lies behind a row's end comes as zeros, so
+  // nothing is read past the weight; a word that begins before the weight is
+  // copied byte by byte.
   static __device__ __forceinline__ void fetch(const RowArgs& a, uint8_t* st, int64_t r0, int k0, int lane) {
     const uint32_t row_bytes = (uint32_t)(a.in / W::BE * W::SB);
     const int r = lane / WORDS, w = lane - r * WORDS;
     if (r >= AT_ONCE) return;
-    const uint8_t* src = a.q + (r0 + r) * row_bytes + k0 / W::BE * W::SB;
-    const uint32_t d = srow(st) + r * PITCH + w * 16;
-    if (r0 > 0 && r0 + kTileR < a.out) {
+    const uint32_t left = row_bytes - k0 / W::BE * W::SB;  // of a row, from k0 on
+    uintptr_t src = reinterpret_cast<uintptr_t>(a.q + (r0 + r) * row_bytes + k0 / W::BE * W::SB) + w * 16;
+    uint32_t d = srow(st) + r * PITCH + w * 16;
+    if (r0 + kTileR <= a.out && left >= WORDS * 16 && (r0 > 0 || k0 > 0)) {
 #pragma unroll
       for (int i = 0; i < kTileR; i += AT_ONCE, src += AT_ONCE * row_bytes)
         if (i + AT_ONCE <= kTileR || i + r < kTileR)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + i * PITCH),
-                       "l"((reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15) + w * 16)
-                       : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + i * PITCH), "l"(src & ~(uintptr_t)15) : "memory");
     } else {
-      const uint8_t* const end = a.q + a.out * row_bytes;
 #pragma unroll 1
-      for (int i = 0; i + r < kTileR && r0 + i + r < a.out; i += AT_ONCE, src += AT_ONCE * row_bytes) {
-        const uint8_t* p = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15) + w * 16;
-        if (p >= a.q && p + 16 <= end) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + i * PITCH), "l"(p) : "memory");
+      for (int i = r; i < kTileR && r0 + i < a.out; i += AT_ONCE, src += AT_ONCE * row_bytes, d += AT_ONCE * PITCH) {
+        const uintptr_t p = src & ~(uintptr_t)15;
+        const int64_t n = (int64_t)(reinterpret_cast<uintptr_t>(a.q) + (r0 + i + 1) * row_bytes) - (int64_t)p;  // to the row's end
+        if (p >= reinterpret_cast<uintptr_t>(a.q)) {
+          const uint32_t size = n >= 16 ? 16 : (n > 0 ? (uint32_t)n : 0);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(size ? p : reinterpret_cast<uintptr_t>(a.q)),
+                       "r"(size)
+                       : "memory");
         } else {
+          uint8_t* const e = st + i * PITCH + w * 16;
 #pragma unroll 1
           for (int b = 0; b < 16; b++)
-            if (p + b >= a.q && p + b < end) st[(i + r) * PITCH + w * 16 + b] = p[b];
+            e[b] = b < n && p + b >= reinterpret_cast<uintptr_t>(a.q) ? *reinterpret_cast<const uint8_t*>(p + b) : 0;
         }
       }
     }
@@ -120,15 +123,23 @@ __device__ __forceinline__ uint32_t shift_down(uint32_t lo, uint32_t hi, uint32_
   return __funnelshift_r(lo, hi, bits);
 }
 
-// Sixteen weights of a row: two code words and their scale as a bfloat16
-// pair.  block: the block's first byte in shared memory, half: the byte of
-// its codes to begin with (0, or 8 in the second half of 32).
+// Where sixteen weights of a row lie in shared memory: the aligned word their
+// codes begin in and the shift that brings them down; for 32-element blocks
+// their block's scale byte.
+struct At16 {
+  uint32_t word, shift, scale;
+};
+// block: the block's first byte, half: the byte of its codes to begin with
+// (0, or 8 in the second half of 32)
+__device__ __forceinline__ At16 at16(uint32_t block, uint32_t half) {
+  return {(block + half) & ~3u, (block + half) * 8, block + 16};
+}
+// their two code words and scale (as a bfloat16 pair), `ahead` bytes further on
 template <int KIND>
-__device__ __forceinline__ void load16(const uint8_t* sm, uint32_t block, uint32_t half, uint32_t w[2], uint32_t& f) {
-  const uint32_t at = block + half, c = at & ~3u, sh = at * 8;
-  const uint32_t v0 = word(sm, c), v1 = word(sm, c + 4), v2 = word(sm, c + 8);
-  const uint32_t sb = W4<KIND>::MX ? sm[block + 16] : shift_down(v2, 0, sh) & 0xffu;
-  w[0] = shift_down(v0, v1, sh), w[1] = shift_down(v1, v2, sh);
+__device__ __forceinline__ void load16(const uint8_t* sm, const At16& at, uint32_t ahead, uint32_t w[2], uint32_t& f) {
+  const uint32_t v0 = word(sm, at.word + ahead), v1 = word(sm, at.word + ahead + 4), v2 = word(sm, at.word + ahead + 8);
+  const uint32_t sb = W4<KIND>::MX ? sm[at.scale + ahead] : shift_down(v2, 0, at.shift) & 0xffu;
+  w[0] = shift_down(v0, v1, at.shift), w[1] = shift_down(v1, v2, at.shift);
   f = word(sm, 256 * 128 + sb * 4);
 }
 // the sixteen weights of two code words, o[i] = weights 2 i and 2 i + 1;
@@ -330,19 +341,18 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_forward_kernel(const RowA
       __syncwarp();
       const uint32_t adv = (uint32_t)s * (256 / W::BE * W::SB), off = at0 + slot * R::BYTES;
       slot = slot + 1 == kDepth ? 0 : slot + 1;
+      // 64 columns are 34 or 36 bytes, 128 a multiple of four: two places a row
+      constexpr uint32_t RUN = 64 / W::BE * W::SB;
       const uint32_t p0 = off + ((sk0 + adv) & 15u), p1 = off + 8 * R::PITCH + ((sk1 + adv) & 15u);
+      const At16 e0[2] = {at16(p0, half), at16(p0 + RUN, half)}, e1[2] = {at16(p1, half), at16(p1 + RUN, half)};
 #pragma unroll 1
-      for (int b = 0; b < 256; b += 128)
+      for (int b = 0; b < 2; b++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const int c = b + 64 * h;
-          load_x(c < 192 ? k0 + c + 64 : next, x[1 - h]);
-          // behind the row's end the elements are zero and the weights those of
-          // the step's first columns (what lies there could be another row's NaN)
-          const uint32_t run = k0 + c < in ? c / 64 * (64 / W::BE * W::SB) : 0 - (16 * t / W::BE * W::SB);
+          load_x(b + h < 2 ? k0 + 128 * b + 64 * h + 64 : next, x[1 - h]);
           uint32_t w0[2], w1[2], f0, f1, o0[8], o1[8];
-          load16<KIND>(sm, p0 + run, half, w0, f0);
-          load16<KIND>(sm, p1 + run, half, w1, f1);
+          load16<KIND>(sm, e0[h], 2 * RUN * b, w0, f0);
+          load16<KIND>(sm, e1[h], 2 * RUN * b, w1, f1);
           decode16(sm, lane4, w0[0], w0[1], f0, o0);
           decode16(sm, lane4, w1[0], w1[1], f1, o1);
 #pragma unroll
@@ -419,7 +429,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
     for (int r = 0; r < 4; r++) {
       const uint32_t block = st + (4 * t + r) * R::PITCH + ((sk + (uint32_t)(n0 + r) * row_bytes) & 15u);
       uint32_t w[2], f;
-      load16<KIND>(sm, block, half, w, f);
+      load16<KIND>(sm, at16(block, half), 0, w, f);
       if (n0 + r >= a.out) w[0] = w[1] = f = 0;  // behind the last row: whatever the stage held
       decode16(sm, lane * 4, w[0], w[1], f, o[r]);
     }
