@@ -190,16 +190,24 @@ def quant_bytes(kind, n):
 
 
 # ---- buffers: numpy arrays (host) or torch tensors (host or CUDA) ----------
+_torch_module = None
+
+
 def _torch():
-    try:
-        import torch  # noqa: F401
-        return torch
-    except ImportError:
-        return None
+    """torch, or None; kept once it is there (an import statement per call is
+    a third of a microsecond)."""
+    global _torch_module
+    if _torch_module is None:
+        try:
+            import torch
+            _torch_module = torch
+        except ImportError:
+            return None
+    return _torch_module
 
 
 def is_torch(x):
-    t = _torch()
+    t = _torch_module or _torch()
     return t is not None and isinstance(x, t.Tensor)
 
 

@@ -21,10 +21,10 @@ __device__ __forceinline__ void previous_done() { asm volatile("griddepcontrol.w
 // ---------------------------------------------------------------------------
 
 // Rows of whole blocks: the weight is one flat run of blocks, so are its
-// bfloat16 values.  A tile of 4096 elements is 2304 or 2176 bytes, copied to
+// bfloat16 values.  A tile of 8192 elements is 4608 or 4352 bytes, copied to
 // shared memory with 16-byte loads; every thread then decodes eight elements
-// twice, so that neighbouring threads write neighbouring 16 bytes.
-constexpr int kUnpackTile = 4096;
+// four times, so that neighbouring threads write neighbouring 16 bytes.
+constexpr int kUnpackTile = 8192;
 template <int KIND>
 __global__ void __launch_bounds__(256) unpack_w4_flat_kernel(const uint8_t* __restrict__ q, int64_t numel,
                                                              uint16_t* __restrict__ out) {

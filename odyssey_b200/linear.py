@@ -123,7 +123,7 @@ def _same_place(x, *others):
     """Buffers of one call live on one device (or all on the host)."""
     for o in others:
         t = L.is_torch(o) and o.is_cuda
-        if t != x.cuda or (t and o.device != x.a.device):
+        if t != x.cuda or (t and o.get_device() != x.a.get_device()):
             raise L.OdysseyError("the buffers of a call must be on one device", L.ERR_ARG)
 
 
@@ -148,11 +148,10 @@ def _flat(a):
     return a if a.is_contiguous() else a.contiguous()
 
 
-def _enqueue(device, call):
-    """call(stream) with the device current and torch's stream on it; raises
-    on a non-zero status."""
+def _enqueue(index, call):
+    """call(stream) with that CUDA device current and torch's stream on it;
+    raises on a non-zero status."""
     t = L._torch()
-    index = device.index
     if index != t.cuda.current_device():
         with t.cuda.device(index):
             return L.check(call(t.cuda.current_stream(index).cuda_stream))
@@ -167,7 +166,7 @@ def _workspace_bytes(device_index, op, rows, out, inn, code):
 
 def _workspace(a, op, rows, out, inn, code):
     """(tensor or None, its address, its bytes) for one call on a's device."""
-    n = _workspace_bytes(a.device.index, op, rows, out, inn, code)
+    n = _workspace_bytes(a.get_device(), op, rows, out, inn, code)
     if n <= 0:
         return None, None, 0
     ws = a.new_empty(n, dtype=L._torch().uint8)
@@ -210,7 +209,7 @@ def _product(name, op, x, w, out, out_dtype, dtype, what):
             alpha = w.tensor_scale
     fn = lib.ody_fp4_linear_on_stream if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad_on_stream
     ws, at, n = _workspace(r.a, op, r.rows, nout, nin, r.code)
-    _enqueue(r.a.device, lambda st: fn(w.kind, data.data_ptr(), ts, alpha, nout, nin, r.ptr, r.code, r.rows, r.ld,
+    _enqueue(r.a.get_device(), lambda st: fn(w.kind, data.data_ptr(), ts, alpha, nout, nin, r.ptr, r.code, r.rows, r.ld,
                                        y.data_ptr(), code, other, at, n, st))
     return y
 
@@ -242,7 +241,7 @@ def save_activation8(x, format="e4m3", dtype=None):
         codes, scales = np.empty((r.rows, g * 32), np.uint8), np.empty((r.rows, g), np.uint8)
     lib = L.lib()
     if r.cuda:
-        _enqueue(r.a.device, lambda st: lib.ody_act8_save_on_stream(fmt, r.ptr, r.code, r.rows, r.cols, r.ld,
+        _enqueue(r.a.get_device(), lambda st: lib.ody_act8_save_on_stream(fmt, r.ptr, r.code, r.rows, r.cols, r.ld,
                                                                     codes.data_ptr(), scales.data_ptr(), st))
     else:
         L.check(lib.ody_act8_save(fmt, r.ptr, r.code, r.rows, r.cols, L.ptr(codes), L.ptr(scales)))
@@ -260,7 +259,7 @@ def load_activation8(a, dtype=None, out=None):
     y = _out(r, out, shape, code, "out")
     lib, fmt = L.lib(), FORMATS8[a.format]
     if r.cuda:
-        _enqueue(codes.device, lambda st: lib.ody_act8_load_on_stream(fmt, codes.data_ptr(), scales.data_ptr(), a.rows,
+        _enqueue(codes.get_device(), lambda st: lib.ody_act8_load_on_stream(fmt, codes.data_ptr(), scales.data_ptr(), a.rows,
                                                                       a.cols, y.data_ptr(), code, a.cols, st))
     else:
         L.check(lib.ody_act8_load(fmt, L.ptr(codes), L.ptr(scales), a.rows, a.cols, L.ptr(y), code))
@@ -292,7 +291,7 @@ def linear_wgrad8(dy, a, add=None, alpha=1.0, out=None, out_dtype=None, dtype=No
     if r.cuda:
         ws, at, n = _workspace(r.a, L.LINEAR_WGRAD, r.rows, r.cols, a.cols, r.code)
         plus = None if add is None else add.data_ptr()
-        _enqueue(r.a.device, lambda st: lib.ody_linear_wgrad8_on_stream(
+        _enqueue(r.a.get_device(), lambda st: lib.ody_linear_wgrad8_on_stream(
             fmt, codes.data_ptr(), scales.data_ptr(), a.rows, a.cols, r.ptr, r.code, r.cols, r.ld, alpha, plus,
             y.data_ptr(), code, at, n, st))
     else:
@@ -307,4 +306,4 @@ def linear_status(device=None):
     calls above do not wait, so they cannot say so themselves)."""
     t = L._torch()
     index = None if device is None else t.device(device).index
-    _enqueue(t.device("cuda", t.cuda.current_device() if index is None else index), L.lib().ody_linear_status)
+    _enqueue(t.cuda.current_device() if index is None else index, L.lib().ody_linear_status)
