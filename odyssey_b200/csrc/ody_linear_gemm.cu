@@ -804,7 +804,7 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
   if (e != cudaSuccess) return e;
   // bfloat16 rows that TMA can read are used where they lie
   const void* abase = a.a;
-  int64_t apitch = a.lda, aplane = up(p.arows * a.lda, 8);
+  int64_t apitch = a.lda, aplane = a.lda;  // one plane: its pitch is never used
   if (a.a_dtype != DT_BF16 || (reinterpret_cast<uintptr_t>(a.a) & 15u) || a.lda % 8) {
     uint16_t* a16 = reinterpret_cast<uint16_t*>(base + p.a_off);
     const int64_t es = a.a_dtype == DT_F32 ? 4 : 2;
@@ -823,7 +823,7 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
   const bool amn = a.op == LIN_WGRAD, bmn = a.op != LIN_FORWARD;
   CUtensorMap ma, mb;
   if ((e = make_map(&ma, abase, p.acols, p.arows, p.planes, apitch, aplane, amn ? kBK : kHalf)) != cudaSuccess) return e;
-  if ((e = make_map(&mb, q16, p.qcols, p.qrows, 1, p.qp, p.qrows * p.qp, bmn ? kBK : kHalf)) != cudaSuccess) return e;
+  if ((e = make_map(&mb, q16, p.qcols, p.qrows, 1, p.qp, p.qp, bmn ? kBK : kHalf)) != cudaSuccess) return e;
   GemmArgs g;
   g.o = a.o;
   g.M = p.M, g.N = p.N;

@@ -544,7 +544,7 @@ cudaError_t launch_few_rows(const LinearArgs& l, int sms, cudaStream_t st) {
   a.q = l.q;
   a.out = l.out, a.in = l.in;
   a.rows = (int)l.rows;
-  a.wide = (reinterpret_cast<uintptr_t>(l.a) & 15u) == 0 && (l.lda * (l.a_dtype == DT_F32 ? 4 : 2)) % 16 == 0;
+  a.wide = (reinterpret_cast<uintptr_t>(l.a) & 15u) == 0 && (l.rows == 1 || (l.lda * (l.a_dtype == DT_F32 ? 4 : 2)) % 16 == 0);
   if (l.kind == Q_MXFP4) return launch_dt<Q_MXFP4>(l, a, sms, st);
   if (l.kind == Q_MXFP4_OCP) return launch_dt<Q_MXFP4_OCP>(l, a, sms, st);
   return launch_dt<Q_NVFP4>(l, a, sms, st);

@@ -574,6 +574,79 @@ def test_wait_that_runs_out_is_reported(ody):
     forward_case(ody, 1, "nvfp4", 300, 256, 512, "bfloat16")
 
 
+def test_first_calls_of_a_process_inside_a_capture(tmp_path):
+    """No call before the capture: kernels, attributes and tensor maps are set
+    up while the stream is being captured."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, odyssey_b200 as ody
+w = ody.QuantizedTensor(torch.zeros(1100 * 1040 // 16 * 9, dtype=torch.uint8, device="cuda"), 7, 1100 * 1040)
+w.data.random_(0, 120, generator=torch.Generator(device="cuda").manual_seed(1))
+xs = [torch.randn(r, 1040, device="cuda") for r in (1, 40, 900)]
+dys = [torch.randn(r, 1100, device="cuda") for r in (1, 40, 900)]
+torch.cuda.synchronize()
+def layer():
+    res = []
+    for x, dy in zip(xs, dys):
+        a = ody.save_activation8(x)
+        res += [ody.fp4_linear(x, w), ody.fp4_linear_dgrad(dy, w), ody.linear_wgrad8(dy, a), ody.load_activation8(a)]
+    return res
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    res = layer()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(res, layer()))
+ody.linear_status()
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stdout + r.stderr
+
+
+def test_refusals_on_device_memory(ody):
+    """What only shows with device pointers: host memory among them, unaligned
+    buffers, a workspace that is missing, too small or unaligned; nothing is
+    launched and the output stays as it was."""
+    from odyssey_b200 import _lib as L
+    lib = L.lib()
+    rng = np.random.default_rng(0)
+    w, _ = make_w(ody, rng, "nvfp4", 1100, 1040)
+    x = torch.randn(900, 1040, device="cuda")
+    y = torch.full((900, 1100), 5.0, device="cuda")
+    need = lib.ody_linear_workspace(L.LINEAR_FORWARD, 900, 1100, 1040, L.F32)
+    assert need > 0
+    ws = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    host = np.zeros(900 * 1100, np.float32)
+
+    def call(q=w.data.data_ptr(), x=x.data_ptr(), y=y.data_ptr(), ts=None, ws=ws.data_ptr(), n=need):
+        return lib.ody_fp4_linear_on_stream(w.kind, q, ts, 1.0, 1100, 1040, x, L.F32, 900, 1040, y, L.F32, 1100, ws, n, st)
+
+    assert call(ws=None) == L.ERR_ARG and call(n=need - 1) == L.ERR_ARG and call(ws=ws.data_ptr() + 16) == L.ERR_ARG
+    assert call(x=host.ctypes.data) == L.ERR_ARG and call(y=host.ctypes.data) == L.ERR_ARG
+    assert call(ts=host.ctypes.data) == L.ERR_ARG and call(ws=host.ctypes.data) == L.ERR_ARG
+    assert call(x=x.data_ptr() + 2) == L.ERR_ARG and call(y=y.data_ptr() + 1) == L.ERR_ARG
+    torch.cuda.synchronize()
+    assert (y == 5.0).all()
+    assert call() == L.OK
+    ody.linear_status()
+    assert torch.equal(y, ody.fp4_linear(x, w))
+    a = ody.save_activation8(x)
+    shifted = torch.empty(a.codes.numel() + 8, dtype=torch.uint8, device="cuda")[8:]
+    with pytest.raises(ody.OdysseyError, match="16-byte aligned"):
+        ody.load_activation8(ody.Activation8(shifted.view(900, -1), a.scales, 900, 1040))
+    with pytest.raises(ody.OdysseyError, match="one device"):
+        ody.linear_wgrad8(torch.randn(900, 8), a)
+    with pytest.raises(ody.OdysseyError, match="one device"):
+        ody.fp4_linear(x.cpu(), w)
+    with pytest.raises(ody.OdysseyError, match="one float32"):
+        ody.fp4_linear(x, ody.QuantizedTensor(w.data, R.NVFP4_TENSOR, w.original_numel, torch.ones(2, device="cuda")))
+
+
 # ---- offsets past 32 bits ---------------------------------------------------
 def test_weight_of_more_than_2_32_elements(ody):
     out, inn = 70001, 65536
