@@ -87,69 +87,6 @@ struct Eight {
   }
 };
 
-// Eight neighbouring elements of the quantised operand: codes in their order
-// (weight i in nibble i ^ 1), scales, and as bfloat16.  Weights of rows that
-// are not a multiple of eight wide may begin at any nibble and reach into a
-// second block.
-template <int OP, int KIND>
-struct EightQ {
-  uint32_t code[OP == LIN_WGRAD ? 2 : 1], scale;  // scale: of the elements before `split`, and 8 bits up the others'
-  int split;
-  // row r, column c; n elements are there (8 where blocks)
-  __device__ __forceinline__ void load(const LinearArgs& p, int64_t groups, int64_t r, int64_t c, int n, bool blocks) {
-    split = 8;
-    if constexpr (OP == LIN_WGRAD) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.q + r * groups * kA8Group + c));
-      code[0] = u.x, code[1] = u.y;
-      scale = __ldg(p.scales + r * groups + c / kA8Group);
-    } else {
-      using W = W4<KIND>;
-      const uint64_t e = (uint64_t)(r * p.in + c);
-      const uint8_t* const blk = p.q + e / W::BE * W::SB;
-      const int i0 = (int)(e % W::BE);
-      if (blocks) {
-        const uint8_t* const s = blk + i0 / 2;
-        uint32_t u[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) u[i] = __ldg(s + i);
-        scale = __ldg(blk + W::SB - 1);
-        code[0] = u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24;
-      } else {
-        uint32_t u[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int j = i0 + i;
-          u[i] = i < n ? __ldg(blk + (j < W::BE ? j / 2 : W::SB + (j - W::BE) / 2)) : 0u;
-        }
-        split = W::BE - i0;
-        scale = __ldg(blk + W::SB - 1);
-        if (split < n) scale |= (uint32_t)__ldg(blk + 2 * W::SB - 1) << 8;
-        code[0] = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) code[0] |= (u[i] >> (i0 + i & 1 ? 0 : 4) & 15u) << (4 * (i ^ 1));
-      }
-    }
-  }
-  __device__ __forceinline__ void store(uint8_t* d) const {
-    uint32_t o[4];
-    if constexpr (OP == LIN_WGRAD) {
-      float v[8];
-      a8_values8<KIND>(make_uint2(code[0], code[1]), scale, v);
-#pragma unroll
-      for (int i = 0; i < 4; i++) o[i] = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
-    } else {
-      w4_raw8<KIND>(code[0], o);
-      const uint32_t f0 = w4_scale_bf16x2<KIND>(scale & 255u), f1 = w4_scale_bf16x2<KIND>(scale >> 8 & 255u);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint32_t f = 2 * i + 1 < split ? f0 : (2 * i >= split ? f1 : __byte_perm(f0, f1, 0x5410));
-        o[i] = mul_bf16x2(mul_bf16x2(o[i], kTwo126), f);
-      }
-    }
-    *reinterpret_cast<uint4*>(d) = make_uint4(o[0], o[1], o[2], o[3]);
-  }
-};
-
 template <bool TRANS>
 __device__ __forceinline__ void ldmatrix4(uint32_t at, uint32_t r[4]) {
   if (TRANS)
@@ -175,7 +112,6 @@ __global__ void __launch_bounds__(256) medium_kernel(const LinearArgs p) {
   const int64_t m0 = tile / tn * kMT, n0 = tile % tn * kMT;
   const uint32_t ranks = cluster_size(), rank = cluster_rank();
   const int64_t steps = (R + kMT - 1) / kMT, s0 = steps * rank / ranks, s1 = steps * (rank + 1) / ranks;
-  const int64_t groups = (p.in + kA8Group - 1) / kA8Group;
   const bool blocks = OP == LIN_WGRAD || p.in % 8 == 0;  // eight columns share a block
   const bool wide = (reinterpret_cast<uintptr_t>(p.a) & 15u) == 0 && p.lda * (DT == DT_F32 ? 4 : 2) % 16 == 0;
   // this thread's part of a tile: eight elements of rows t / 8 and t / 8 + 32
@@ -192,7 +128,7 @@ __global__ void __launch_bounds__(256) medium_kernel(const LinearArgs p) {
       a[i].load(p.a, ar * p.lda + ac, ar < (AR ? M : R) ? (int)max((int64_t)0, min((int64_t)8, (AR ? R : M) - ac)) : 0, wide);
       const int64_t br = (BR ? n0 : s * kMT) + row + 32 * i, bc = (BR ? s * kMT : n0) + col;
       on[i] = br < (BR ? N : R) && bc < p.in;
-      if (on[i]) b[i].load(p, groups, br, bc, (int)min((int64_t)8, p.in - bc), blocks);
+      if (on[i]) b[i].load(p.q, p.scales, p.in, br, bc, (int)min((int64_t)8, p.in - bc), blocks);
     }
   };
   const auto store = [&](int to) {

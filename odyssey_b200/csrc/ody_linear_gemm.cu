@@ -4,6 +4,8 @@
 #include <cuda.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "ody_linear_dev.cuh"
 #include "ody_linear_gemm.h"
 
@@ -66,17 +68,12 @@ __global__ void __launch_bounds__(256) unpack_w4_rows_kernel(const uint8_t* __re
                                                              int64_t kp, uint16_t* __restrict__ out) {
   let_next_start();
   const int64_t n = rows * (kp / 8), stride = (int64_t)gridDim.x * blockDim.x;
+  const bool blocks = cols % 8 == 0;  // eight columns share a block
   for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < n; t += stride) {
     const int64_t r = t / (kp / 8), c = (t - r * (kp / 8)) * 8;
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float a = c + 2 * i < cols ? W4<KIND>::at(q, r * cols + c + 2 * i) : 0.0f;
-      const float b = c + 2 * i + 1 < cols ? W4<KIND>::at(q, r * cols + c + 2 * i + 1) : 0.0f;
-      // the product is exact in bfloat16, so its upper half is all of it
-      o[i] = (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xffff0000u);
-    }
-    *reinterpret_cast<uint4*>(out + r * kp + c) = make_uint4(o[0], o[1], o[2], o[3]);
+    EightQ<LIN_FORWARD, KIND> e;
+    e.load(q, nullptr, cols, r, c, (int)min((int64_t)8, cols - c), blocks);
+    e.store(reinterpret_cast<uint8_t*>(out + r * kp + c));
   }
 }
 
@@ -189,8 +186,7 @@ __global__ void __launch_bounds__(256) pack_planes_kernel(const void* __restrict
 constexpr int kBM = 256, kBN = 256, kBK = 64, kStages = 6;
 constexpr int kHalf = 128;                                   // rows of A and of B in each CTA
 constexpr int kHalfBytes = kHalf * kBK * 2, kStageBytes = 2 * kHalfBytes;
-constexpr int kStagePitch = 33;                              // floats; the epilogue's 32 x 32 transposes
-constexpr int kEpiBytes = 8 * 32 * kStagePitch * 4;
+constexpr int kEpiBytes = 8 * 32 * 32 * 4;                   // the epilogue's 32 x 32 transposes
 constexpr int kGemmSmem = kStages * kStageBytes + kEpiBytes + 1024;
 constexpr int kGemmThreads = 384;
 // bound on every wait, in cycles of the SM's counter: 2 s at 2 GHz
@@ -323,43 +319,72 @@ struct Pieces {
   }
 };
 
-// 32 x 32 results (at c, in rows of ld) out of a warp's transposing buffer
-__device__ __forceinline__ void store_block(const float* buf, void* c, const void* add, int dtype, int64_t ld, float scale,
-                                            int rows, int cols, int lane) {
-  const int es = dtype == DT_F32 ? 4 : 2;
-  if (dtype != DT_F32 && !add && cols >= 32 && ((reinterpret_cast<uintptr_t>(c) | (uintptr_t)(ld * 2)) & 3u) == 0) {
-    // 16-bit results in pairs, two rows at a time
-    const int k = (lane & 15) * 2, r0 = lane >> 4;
-    const float* s = buf + r0 * kStagePitch + k;
-    uint16_t* d = reinterpret_cast<uint16_t*>(c) + r0 * ld + k;
-    const bool half = dtype == DT_F16;
-#pragma unroll 4
-    for (int i = r0; i < rows; i += 2, s += 2 * kStagePitch, d += 2 * ld) {
-      const float a = __fmul_rn(s[0], scale), b = __fmul_rn(s[1], scale);
-      *reinterpret_cast<uint32_t*>(d) = half ? f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16
-                                             : f32_to_bf16_bits(a) | (uint32_t)f32_to_bf16_bits(b) << 16;
+// A warp's 32 x 32 results, one row per lane, turned in shared memory (rows of
+// 128 bytes, their 16-byte pieces exchanged by the row's number so that
+// neither side meets a bank twice) and stored at c, rows of ld.
+__device__ __forceinline__ float4* piece_of(float* buf, int row, int piece) {
+  return reinterpret_cast<float4*>(buf) + row * 8 + (piece ^ (row & 7));
+}
+template <int DT>
+__device__ __forceinline__ void store_block(float* buf, void* c, const void* add, int64_t ld, float scale, int rows, int cols,
+                                            int lane) {
+  constexpr int ES = DT == DT_F32 ? 4 : 2;
+  const auto bits = [](float v) { return DT == DT_F16 ? f32_to_f16_bits(v) : f32_to_bf16_bits(v); };
+  if (cols >= 32 && ((reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(add) | (uintptr_t)(ld * ES)) &
+                     (uintptr_t)(4 * ES - 1)) == 0) {
+    // four columns per lane, four rows at a time
+    const int64_t at = ((lane >> 3) * ld + (lane & 7) * 4) * ES;
+    uint8_t* d = reinterpret_cast<uint8_t*>(c) + at;
+    const uint8_t* e = reinterpret_cast<const uint8_t*>(add) + at;
+#pragma unroll 2
+    for (int r = lane >> 3; r < rows; r += 4, d += 4 * ld * ES, e += 4 * ld * ES) {
+      float4 v = *piece_of(buf, r, lane & 7);
+      v.x = __fmul_rn(v.x, scale), v.y = __fmul_rn(v.y, scale), v.z = __fmul_rn(v.z, scale), v.w = __fmul_rn(v.w, scale);
+      if (add) {
+        float w[4];
+        if constexpr (DT == DT_F32) {
+          const float4 f = *reinterpret_cast<const float4*>(e);
+          w[0] = f.x, w[1] = f.y, w[2] = f.z, w[3] = f.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(e);
+          const uint16_t h[4] = {(uint16_t)u.x, (uint16_t)(u.x >> 16), (uint16_t)u.y, (uint16_t)(u.y >> 16)};
+#pragma unroll
+          for (int k = 0; k < 4; k++) w[k] = DT == DT_F16 ? f16_bits_to_f32(h[k]) : bf16_bits_to_f32(h[k]);
+        }
+        v.x = __fadd_rn(v.x, w[0]), v.y = __fadd_rn(v.y, w[1]), v.z = __fadd_rn(v.z, w[2]), v.w = __fadd_rn(v.w, w[3]);
+      }
+      if constexpr (DT == DT_F32)
+        *reinterpret_cast<float4*>(d) = v;
+      else
+        *reinterpret_cast<uint2*>(d) =
+            make_uint2(bits(v.x) | (uint32_t)bits(v.y) << 16, bits(v.z) | (uint32_t)bits(v.w) << 16);
     }
   } else if (lane < cols) {
-    c = reinterpret_cast<uint8_t*>(c) + lane * es;
-    if (!add && dtype == DT_F32) {
-#pragma unroll 4
-      for (int r = 0; r < rows; r++) reinterpret_cast<float*>(c)[r * ld] = __fmul_rn(buf[r * kStagePitch + lane], scale);
-    } else {
-      // what is added comes in eight rows at a time: one by one, every store
-      // would wait for a load (add may be c, so they are not reordered)
+    // any alignment: a column per lane; what is added comes four rows at a time
+    uint8_t* d = reinterpret_cast<uint8_t*>(c) + lane * ES;
+    const uint8_t* e = reinterpret_cast<const uint8_t*>(add) + lane * ES;
+    const int64_t step = ld * ES;
 #pragma unroll 1
-      for (int r = 0; r < rows; r += 8) {
-        float w[8];
+    for (int r = 0; r < rows; r += 4, d += 4 * step, e += 4 * step) {
+      float v[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = add && r + i < rows ? load_elem(add, dtype, (r + i) * ld + lane) : 0.0f;
+      for (int k = 0; k < 4; k++)
+        v[k] = __fmul_rn(reinterpret_cast<const float*>(piece_of(buf, r + k, lane >> 2))[lane & 3], scale);
+      if (add) {
+        float w[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-          if (r + i < rows) {
-            float x = __fmul_rn(buf[(r + i) * kStagePitch + lane], scale);
-            if (add) x = __fadd_rn(x, w[i]);
-            store_elem(c, dtype, (r + i) * ld, x);
-          }
+        for (int k = 0; k < 4; k++) w[k] = r + k < rows ? load_elem(e + k * step, DT, 0) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = __fadd_rn(v[k], w[k]);
       }
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (r + k < rows) {
+          if constexpr (DT == DT_F32)
+            *reinterpret_cast<float*>(d + k * step) = v[k];
+          else
+            *reinterpret_cast<uint16_t*>(d + k * step) = bits(v[k]);
+        }
     }
   }
 }
@@ -377,7 +402,7 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t v[32]) {
 }
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-template <bool AMN, bool BMN>
+template <bool AMN, bool BMN, int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const GemmArgs g) {
   extern __shared__ uint8_t dyn[];
@@ -486,8 +511,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + half * (kBN / 2);
     const uint32_t done = in_cta(tempty, 0);
-    float* buf32 = reinterpret_cast<float*>(dyn + (smem - sptr(dyn)) + kStages * kStageBytes) + (warp - 4) * 32 * kStagePitch;
+    float* buf32 = reinterpret_cast<float*>(dyn + (smem - sptr(dyn)) + kStages * kStageBytes) + (warp - 4) * 32 * 32;
     const float scale = out_scale(g.o);
+    constexpr int ES = DT == DT_F32 ? 4 : 2;
     int chunk = 0;
     bool ok = true;
     Pieces w(g, pair);
@@ -519,32 +545,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
       if (!ok) break;
       const int64_t m0 = (int64_t)tm * kBM + rank * kHalf + quarter * 32, n0 = (int64_t)tn * kBN + half * (kBN / 2);
       if (m0 >= g.M || n0 >= g.N) continue;
-      void* c;
-      const void* add = nullptr;
-      int dtype = DT_F32;
-      int64_t ld = kBN;
-      float sc = 1.0f;
-      if (w.s1 - w.s0 < g.total) {  // a piece of a shared tile
-        c = g.partial + (int64_t)(2 * pair + (w.s0 == 0)) * kBM * kBN + (rank * kHalf + quarter * 32) * kBN + half * (kBN / 2);
+      const bool part = w.s1 - w.s0 < g.total;  // of a shared tile
+      const int rows = (int)min((int64_t)32, g.M - m0);
+      uint8_t* c;
+      const uint8_t* add = nullptr;
+      if (part) {
+        c = reinterpret_cast<uint8_t*>(g.partial + (int64_t)(2 * pair + (w.s0 == 0)) * kBM * kBN +
+                                       (rank * kHalf + quarter * 32) * kBN + half * (kBN / 2));
       } else {
-        dtype = g.o.dtype, ld = g.o.ld, sc = scale;
-        const int64_t at = (m0 * ld + n0) * (dtype == DT_F32 ? 4 : 2);
+        const int64_t at = (m0 * g.o.ld + n0) * ES;
         c = reinterpret_cast<uint8_t*>(g.o.c) + at;
         if (g.o.add) add = reinterpret_cast<const uint8_t*>(g.o.add) + at;
       }
-      const int rows = (int)min((int64_t)32, g.M - m0), es = dtype == DT_F32 ? 4 : 2;
-      int cols = (int)min((int64_t)(kBN / 2), g.N - n0);
 #pragma unroll 1
-      for (; cols > 0; cols -= 32) {
+      for (int cols = (int)min((int64_t)(kBN / 2), g.N - n0); cols > 0; cols -= 32) {
 #pragma unroll
-        for (int i = 0; i < 32; i++) buf32[lane * kStagePitch + i] = acc[i];
+        for (int i = 0; i < 8; i++)
+          *piece_of(buf32, lane, i) = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
 #pragma unroll
         for (int i = 0; i < kBN / 2 - 32; i++) acc[i] = acc[i + 32];
         __syncwarp();
-        store_block(buf32, c, add, dtype, ld, sc, rows, cols, lane);
+        if (part) {
+          store_block<DT_F32>(buf32, c, nullptr, kBN, 1.0f, rows, 32, lane);  // whole: its place is 256 wide
+          c += 32 * 4;
+        } else {
+          store_block<DT>(buf32, c, add, g.o.ld, scale, rows, cols, lane);
+          c += 32 * ES;
+          if (add) add += 32 * ES;
+        }
         __syncwarp();
-        c = reinterpret_cast<uint8_t*>(c) + 32 * es;
-        if (add) add = reinterpret_cast<const uint8_t*>(add) + 32 * es;
       }
     }
   }
@@ -741,21 +770,21 @@ cudaError_t unpack_w4(const LinearArgs& a, const Plan& p, uint16_t* out, int sms
   return cudaGetLastError();
 }
 
-template <bool AMN, bool BMN>
+template <bool AMN, bool BMN, int DT>
 cudaError_t run_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& g, int sms, cudaStream_t st) {
   static bool set[64] = {false};  // per device; setting it twice is harmless
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !set[dev]) {
     const cudaError_t e =
-        cudaFuncSetAttribute(gemm_kernel<AMN, BMN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
+        cudaFuncSetAttribute(gemm_kernel<AMN, BMN, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
   // with whole tiles only, no more pairs than tiles
   const int64_t shares = ((int64_t)g.shared * g.total + g.deal - 1) / g.deal;
   const int64_t work = g.tiles_m * (int64_t)g.tiles_n > g.shared ? sms / 2 : shares;
-  return launch_next(gemm_kernel<AMN, BMN>, dim3((unsigned)std::min<int64_t>(work, sms / 2) * 2), kGemmThreads, kGemmSmem,
+  return launch_next(gemm_kernel<AMN, BMN, DT>, dim3((unsigned)std::min<int64_t>(work, sms / 2) * 2), kGemmThreads, kGemmSmem,
                      st, ma, mb, g);
 }
 
@@ -831,12 +860,14 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
   g.steps = p.steps, g.total = p.steps * p.planes, g.chunk = a.o.dtype == DT_F32 ? 8 : 16;
   g.shared = p.shared, g.deal = p.deal;
   g.partial = reinterpret_cast<float*>(base + p.p_off);
-  if (a.op == LIN_FORWARD)
-    e = run_gemm<false, false>(ma, mb, g, sms, st);
-  else if (a.op == LIN_DGRAD)
-    e = run_gemm<false, true>(ma, mb, g, sms, st);
-  else
-    e = run_gemm<true, true>(ma, mb, g, sms, st);
+  const auto run = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (a.op == LIN_FORWARD) return run_gemm<false, false, DT>(ma, mb, g, sms, st);
+    return a.op == LIN_DGRAD ? run_gemm<false, true, DT>(ma, mb, g, sms, st) : run_gemm<true, true, DT>(ma, mb, g, sms, st);
+  };
+  e = a.o.dtype == DT_F32   ? run(std::integral_constant<int, DT_F32>())
+      : a.o.dtype == DT_F16 ? run(std::integral_constant<int, DT_F16>())
+                            : run(std::integral_constant<int, DT_BF16>());
   if (e != cudaSuccess || !p.split) return e;
   return launch_next(gemm_join_kernel, dim3((unsigned)p.shared * 32), 256, 0, st, g);
 }
