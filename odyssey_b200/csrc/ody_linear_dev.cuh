@@ -13,13 +13,6 @@ struct W4 {
   static constexpr int BE = MX ? 32 : 16;  // elements per block
   static constexpr int SB = MX ? 17 : 9;   // bytes per block
 
-  // a block's scale: E8M0 (in the OCP kind 0 is 2^-127 and 255 NaN) or E4M3
-  static __device__ __forceinline__ float scale(uint32_t b) {
-    if (KIND == Q_MXFP4_OCP)
-      return b == 0xFF ? __uint_as_float(0x7fc00000u) : (b ? __uint_as_float(b << 23) : __uint_as_float(0x00400000u));
-    if (KIND == Q_MXFP4) return e8m0_to_f32((uint8_t)b);
-    return e4m3_to_f32((uint8_t)b);
-  }
   // code times scale; exact in float32 and, for finite scales, in bfloat16:
   // two bits of value times at most four of scale.  Code 1 is 0.5 in the OCP
   // kind and 0 in the others, and their zero is not multiplied by the scale.
@@ -32,12 +25,6 @@ struct W4 {
     }
     return fp4_decode(code, sf);
   }
-  static __device__ __forceinline__ float at(const uint8_t* q, int64_t e) {
-    const uint8_t* blk = q + (e / BE) * SB;
-    const int i = (int)(e % BE);
-    const uint32_t b = blk[i >> 1];
-    return value(i & 1 ? b & 15u : b >> 4, scale(blk[SB - 1]));
-  }
 };
 
 // ---- eight weights at once, as bfloat16 pairs -------------------------------
@@ -46,7 +33,8 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// the block scale as a bfloat16 pair (exact)
+// a block's scale as a bfloat16 pair (exact): E8M0 (in the OCP kind 0 is
+// 2^-127 and 255 NaN) or E4M3
 template <int KIND>
 __device__ __forceinline__ uint32_t w4_scale_bf16x2(uint32_t byte) {
   uint32_t h;

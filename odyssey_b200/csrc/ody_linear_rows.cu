@@ -45,6 +45,7 @@ struct RowArgs {
   int64_t out, in;  // weight rows and columns
   int rows;         // of a
   int wide;         // a's rows are 16-byte aligned
+  int keep;         // dgrad: a warp has more than 32 steps
 };
 
 // A warp's ring of weight tiles, 16 rows x K columns each.  A row's piece is
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_forward_kernel(const RowA
   for (; tile < tiles; tile += tile_stride) {
     const int64_t r0 = tile * kTileR;
     const uint32_t sk0 = q0 + (uint32_t)(r0 + g) * row_bytes, sk1 = sk0 + 8 * row_bytes;
-    float acc[NT][4] = {};
+    float acc[NT][4] = {}, part[NT][4] = {};  // part: of two steps, 32 mma (a tensor core cuts low bits off)
 #pragma unroll 1
     for (int i = 0; i < mine; i++) {
       const int s = me + i * stride, k0 = s * 256 + 16 * t;
@@ -359,8 +360,14 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_forward_kernel(const RowA
           for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int j = 0; j < 8; j += 2)
-              mma16816(acc[n], o0[j], o1[j], o0[j + 1], o1[j + 1], x[h][n][j], x[h][n][j + 1]);
+              mma16816(part[n], o0[j], o1[j], o0[j + 1], o1[j + 1], x[h][n][j], x[h][n][j + 1]);
         }
+      if ((i & 1) || i + 1 == mine) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) acc[n][j] = __fadd_rn(acc[n][j], part[n][j]), part[n][j] = 0.0f;
+      }
     }
     // red: [warp][weight row][column], an odd pitch
 #pragma unroll
@@ -391,7 +398,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
   const int64_t k0 = (int64_t)(blockIdx.x / cluster_size()) * kDK;
   const int64_t steps = (a.out + kTileR - 1) / kTileR, stride = (int64_t)kRowWarps * cluster_size();
   uint8_t* const ring = sm + kTableBytes + warp * kDepth * R::BYTES;
-  float acc[8][NT][4] = {};
+  // A warp's sums, [column][17 floats per 16 k].  Where it has more than 32
+  // steps they have a place of their own and take the accumulators in every
+  // 32 mma (a tensor core cuts low bits off); else they lie where the ring was.
+  float* const sums = reinterpret_cast<float*>(sm + (a.keep ? kTableBytes + kRowWarps * kDepth * R::BYTES : 0));
   int64_t ahead = (int64_t)cluster_rank() * kRowWarps + warp;
   uint32_t y[NT][2];  // of the next step
   Column<DT> cols[NT];
@@ -407,54 +417,63 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
   // this lane's 16 columns: a block, or half a block of 32
   const uint32_t at0 = kTableBytes + warp * kDepth * R::BYTES + 16 * g / W::BE * W::SB, half = 16 * g % W::BE / 2;
   int slot = 0;
+  int64_t s = ahead - (kDepth - 1) * stride;
+  bool first = true;
 #pragma unroll 1
-  for (int64_t s = ahead - (kDepth - 1) * stride; s < steps;
-       s += stride, ahead += stride, slot = slot + 1 == kDepth ? 0 : slot + 1) {
-    __syncwarp();  // all lanes are done with the stage that is filled next
-    if (ahead < steps) R::fetch(a, ring + slot * R::BYTES, ahead * kTileR, (int)k0, lane);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    if (s < 0) continue;
-    uint32_t z[NT][2];
+  do {
+    float acc[8][NT][4] = {};
+    const int64_t end = a.keep ? min(steps, s + 32 * stride) : steps;
+#pragma unroll 1
+    for (; s < end; s += stride, ahead += stride, slot = slot + 1 == kDepth ? 0 : slot + 1) {
+      __syncwarp();  // all lanes are done with the stage that is filled next
+      if (ahead < steps) R::fetch(a, ring + slot * R::BYTES, ahead * kTileR, (int)k0, lane);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (s < 0) continue;
+      uint32_t z[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-      z[n][0] = y[n][0], z[n][1] = y[n][1];
-      cols[n].load((s + stride) * kTileR + 4 * t, a.out, a.wide, y[n]);
+      for (int n = 0; n < NT; n++) {
+        z[n][0] = y[n][0], z[n][1] = y[n][1];
+        cols[n].load((s + stride) * kTileR + 4 * t, a.out, a.wide, y[n]);
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      __syncwarp();
+      const uint32_t st = at0 + (slot + 1 == kDepth ? 0 : slot + 1) * R::BYTES;
+      const int64_t n0 = s * kTileR + 4 * t;
+      uint32_t o[4][8];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const uint32_t block = st + (4 * t + r) * R::PITCH + ((sk + (uint32_t)(n0 + r) * row_bytes) & 15u);
+        uint32_t w[2], f;
+        load16<KIND>(sm, at16(block, half), 0, w, f);
+        if (n0 + r >= a.out) w[0] = w[1] = f = 0;  // behind the last row: whatever the stage held
+        decode16(sm, lane * 4, w[0], w[1], f, o[r]);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        const uint32_t a0 = __byte_perm(o[0][q], o[1][q], 0x5410), a1 = __byte_perm(o[0][q], o[1][q], 0x7632);
+        const uint32_t a2 = __byte_perm(o[2][q], o[3][q], 0x5410), a3 = __byte_perm(o[2][q], o[3][q], 0x7632);
+#pragma unroll
+        for (int n = 0; n < NT; n++) mma16816(acc[q][n], a0, a1, a2, a3, z[n][0], z[n][1]);
+      }
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-    __syncwarp();
-    const uint32_t st = at0 + (slot + 1 == kDepth ? 0 : slot + 1) * R::BYTES;
-    const int64_t n0 = s * kTileR + 4 * t;
-    uint32_t o[4][8];
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const uint32_t block = st + (4 * t + r) * R::PITCH + ((sk + (uint32_t)(n0 + r) * row_bytes) & 15u);
-      uint32_t w[2], f;
-      load16<KIND>(sm, at16(block, half), 0, w, f);
-      if (n0 + r >= a.out) w[0] = w[1] = f = 0;  // behind the last row: whatever the stage held
-      decode16(sm, lane * 4, w[0], w[1], f, o[r]);
+    if (s >= steps) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncthreads();
     }
 #pragma unroll
-    for (int q = 0; q < 8; q++) {
-      const uint32_t a0 = __byte_perm(o[0][q], o[1][q], 0x5410), a1 = __byte_perm(o[0][q], o[1][q], 0x7632);
-      const uint32_t a2 = __byte_perm(o[2][q], o[3][q], 0x5410), a3 = __byte_perm(o[2][q], o[3][q], 0x7632);
+    for (int q = 0; q < 8; q++)
 #pragma unroll
-      for (int n = 0; n < NT; n++) mma16816(acc[q][n], a0, a1, a2, a3, z[n][0], z[n][1]);
-    }
-  }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  float* red = reinterpret_cast<float*>(sm);  // [warp][column][17 floats per 16 k]
+      for (int n = 0; n < NT; n++) {
+        float* d = sums + (warp * C + n * 8 + 2 * t) * kRedPitch + 17 * g + 2 * q;
+        float* const at[4] = {d, d + kRedPitch, d + 1, d + kRedPitch + 1};
 #pragma unroll
-  for (int q = 0; q < 8; q++)
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      float* d = red + (warp * C + n * 8 + 2 * t) * kRedPitch + 17 * g + 2 * q;
-      d[0] = acc[q][n][0], d[kRedPitch] = acc[q][n][1];
-      d[1] = acc[q][n][2], d[kRedPitch + 1] = acc[q][n][3];
-    }
+        for (int i = 0; i < 4; i++) *at[i] = first ? acc[q][n][i] : __fadd_rn(*at[i], acc[q][n][i]);
+      }
+    first = false;
+  } while (s < steps);
   const float scale = out_scale(a.o);
   add_and_store<kRowWarps>(
-      red, C * kRedPitch, kDK * a.rows, P, kRedPitch,
+      sums, C * kRedPitch, kDK * a.rows, P, kRedPitch,
       [&](int o) { return (o >> 7) * P * kRedPitch + 17 * ((o & 127) >> 4) + (o & 15); },
       [&](int o, float v) {
         if (k0 + (o & 127) < a.in) finish(a.o, scale, o >> 7, k0 + (o & 127), v);
@@ -466,27 +485,30 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
 // ---------------------------------------------------------------------------
 namespace {
 
-template <void (*kernel)(const RowArgs)>
-cudaError_t launch_rows(const RowArgs& a, int64_t tiles, bool walked, int64_t steps, int smem, int sms,
-                        cudaStream_t st) {
-  static bool set[64] = {false};  // of this kernel, per device; setting it twice is harmless
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) set[dev] = true;
-  }
-  // two CTAs per SM; fewer tiles than that are shared by clusters while every
-  // CTA still has a step for its warps
+// CTAs that share a tile: two per SM are launched, and fewer tiles than that
+// are shared while every CTA still has a step for its warps
+int cluster_for(int64_t tiles, int64_t steps, int sms) {
   int cluster = 1;
   while (cluster < 8 && tiles * cluster * 2 <= 2 * sms && cluster < steps) cluster *= 2;
+  return cluster;
+}
+
+template <void (*kernel)(const RowArgs)>
+cudaError_t launch_rows(const RowArgs& a, int64_t grid, int cluster, int smem, cudaStream_t st) {
+  static int most[64] = {0};  // of this kernel, per device; setting it twice is harmless
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || most[dev] < smem) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) most[dev] = smem;
+  }
   if (cluster == 1) {
-    kernel<<<(unsigned)(walked ? std::min<int64_t>(tiles, 2 * sms) : tiles), kRowThreads, smem, st>>>(a);
+    kernel<<<(unsigned)grid, kRowThreads, smem, st>>>(a);
     return cudaGetLastError();
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((walked ? std::min<int64_t>(tiles, 2 * sms) : tiles) * cluster));
+  cfg.gridDim = dim3((unsigned)(grid * cluster));
   cfg.blockDim = dim3(kRowThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -498,18 +520,20 @@ cudaError_t launch_rows(const RowArgs& a, int64_t tiles, bool walked, int64_t st
 }
 
 template <int KIND, int DT, int NT>
-cudaError_t launch_one(const LinearArgs& l, const RowArgs& a, int sms, cudaStream_t st) {
-  const int64_t columns = (a.in + 255) / 256, rows = (a.out + kTileR - 1) / kTileR;
-  if (l.op == LIN_FORWARD)
+cudaError_t launch_one(const LinearArgs& l, RowArgs a, int sms, cudaStream_t st) {
+  const int64_t rows = (a.out + kTileR - 1) / kTileR;
+  if (l.op == LIN_FORWARD) {
+    const int cluster = cluster_for(rows, (a.in + 256 * kRowWarps - 1) / (256 * kRowWarps), sms);
     return launch_rows<rows_forward_kernel<KIND, DT, NT>>(
-        a, rows, true, (columns + kRowWarps - 1) / kRowWarps,
-        kTableBytes + kRowWarps * kForwardDepth<NT> * Ring<KIND, 256>::BYTES + kRowWarps * kTileR * (NT * 8 + 1) * 4, sms,
-        st);
+        a, std::min<int64_t>(rows, 2 * sms), cluster,
+        kTableBytes + kRowWarps * kForwardDepth<NT> * Ring<KIND, 256>::BYTES + kRowWarps * kTileR * (NT * 8 + 1) * 4, st);
+  }
   if constexpr (NT <= 2) {
+    constexpr int ring = kTableBytes + kRowWarps * kDepth * Ring<KIND, kDK>::BYTES, sums = kRowWarps * NT * 8 * kRedPitch * 4;
     const int64_t tiles = (a.in + kDK - 1) / kDK;
-    return launch_rows<rows_dgrad_kernel<KIND, DT, NT>>(
-        a, tiles, false, (rows + kRowWarps - 1) / kRowWarps,
-        std::max(kTableBytes + kRowWarps * kDepth * Ring<KIND, kDK>::BYTES, kRowWarps * NT * 8 * kRedPitch * 4), sms, st);
+    const int cluster = cluster_for(tiles, (rows + kRowWarps - 1) / kRowWarps, sms);
+    a.keep = rows > 32 * (int64_t)kRowWarps * cluster;
+    return launch_rows<rows_dgrad_kernel<KIND, DT, NT>>(a, tiles, cluster, a.keep ? ring + sums : std::max(ring, sums), st);
   }
   return cudaErrorInvalidValue;
 }
@@ -544,6 +568,7 @@ cudaError_t launch_few_rows(const LinearArgs& l, int sms, cudaStream_t st) {
   a.q = l.q;
   a.out = l.out, a.in = l.in;
   a.rows = (int)l.rows;
+  a.keep = 0;
   a.wide = (reinterpret_cast<uintptr_t>(l.a) & 15u) == 0 && (l.rows == 1 || (l.lda * (l.a_dtype == DT_F32 ? 4 : 2)) % 16 == 0);
   if (l.kind == Q_MXFP4) return launch_dt<Q_MXFP4>(l, a, sms, st);
   if (l.kind == Q_MXFP4_OCP) return launch_dt<Q_MXFP4_OCP>(l, a, sms, st);

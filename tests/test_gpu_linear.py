@@ -93,6 +93,14 @@ def test_large_products(ody, rows, out, inn, dgrad):
         forward_case(ody, rows + i, kind, rows, out, inn, dtype, out_dtype, dgrad, pad=(0, 0, 8, 9)[i])
 
 
+@pytest.mark.parametrize("rows,out,inn", [(2, 40, 33024), (1, 2500, 10304), (9, 4300, 19072), (3, 70000, 64), (12, 34000, 160)])
+@pytest.mark.parametrize("dgrad", [False, True], ids=["forward", "dgrad"])
+def test_few_rows_long_reductions(ody, rows, out, inn, dgrad):
+    """More than 32 tensor-core steps in a warp's sum, with and without clusters."""
+    forward_case(ody, rows, "nvfp4", rows, out, inn, "bfloat16", "float32", dgrad)
+    forward_case(ody, rows, "mxfp4", min(rows, 5), out, inn, "float32", None, dgrad)
+
+
 @pytest.mark.parametrize("out_dtype", DTYPES)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_product_types_and_pitches(ody, dtype, out_dtype):
