@@ -46,74 +46,98 @@ struct RowArgs {
   int rows;         // of a
   int wide;         // a's rows are 16-byte aligned
   int keep;         // dgrad: a warp has more than 32 steps
+  int cluster;      // forward: log2 of the CTAs of a cluster,
+  int per, extra;   // rows / 8 of a cluster's run, and how many runs have one more
 };
 
-// A warp's ring of weight tiles, 16 rows x K columns each.  A row's piece is
+// A warp's ring of weight tiles, ROWS rows x K columns each.  A row's piece is
 // at most K * 9 / 16 bytes at any byte offset, so it is copied as the aligned
-// 16-byte words around it.  For 256 columns the pitch of eleven words keeps a
-// warp's reads, eight rows by four offsets of nine words, on 32 banks.
-template <int KIND, int K>
+// 16-byte words around it.  An odd pitch in words spreads a warp's reads,
+// eight rows by four offsets, over the banks.
+template <int KIND, int K, int ROWS>
 struct Ring {
   using W = W4<KIND>;
-  static constexpr int WORDS = (K * 9 / 16 + 30) / 16, PITCH = (WORDS | 1) * 16, BYTES = kTileR * PITCH;
+  static constexpr int WORDS = (K * 9 / 16 + 30) / 16, PITCH = (WORDS | 1) * 16, BYTES = ROWS * PITCH;
   static constexpr int AT_ONCE = 32 / WORDS;  // rows that one copy of every lane takes
   static_assert(K % 128 == 0, "whole blocks");
 
-  // Columns k0.. of rows r0.. into a stage; neighbouring lanes copy
-  // neighbouring words of a row (two lanes to a row, each with every other
-  // word, halved the rate).  What lies behind a row's end comes as zeros, so
-  // nothing is read past the weight; a word that begins before the weight is
-  // copied byte by byte.
-  static __device__ __forceinline__ void fetch(const RowArgs& a, uint8_t* st, int64_t r0, int k0, int lane) {
+  // where this lane's row and word of rows r0.. begin
+  static __device__ __forceinline__ uintptr_t place(const RowArgs& a, int64_t r0, int lane) {
+    return reinterpret_cast<uintptr_t>(a.q) + (r0 + lane / WORDS) * (a.in / W::BE * W::SB) + lane % WORDS * 16;
+  }
+  // Columns k0.. (`before` bytes into their rows) of n rows r0.. into a stage,
+  // from place(r0); neighbouring lanes copy neighbouring words of a row (two
+  // lanes to a row, each with every other word, halved the rate).  What lies
+  // behind a row's end comes as zeros where its columns are used, so nothing
+  // is read past the weight; a word that begins before the weight is copied
+  // byte by byte.
+  static __device__ __forceinline__ void fetch(const RowArgs& a, uint8_t* st, uintptr_t from, int r0, int n, int k0,
+                                               uint32_t before, int lane) {
     const uint32_t row_bytes = (uint32_t)(a.in / W::BE * W::SB);
-    const int r = lane / WORDS, w = lane - r * WORDS;
+    const uint64_t more = (uint64_t)AT_ONCE * row_bytes;
+    const int r = lane / WORDS;
     if (r >= AT_ONCE) return;
-    const uint32_t left = row_bytes - k0 / W::BE * W::SB;  // of a row, from k0 on
-    uintptr_t src = reinterpret_cast<uintptr_t>(a.q + (r0 + r) * row_bytes + k0 / W::BE * W::SB) + w * 16;
-    uint32_t d = srow(st) + r * PITCH + w * 16;
-    if (r0 + kTileR <= a.out && left >= WORDS * 16 && (r0 > 0 || k0 > 0)) {
+    const uintptr_t q = reinterpret_cast<uintptr_t>(a.q);
+    from += before;
+    uint32_t d = srow(st) + r * PITCH + lane % WORDS * 16;
+    if (k0 <= (int)a.in - K && (r0 + n < (int)a.out || before + WORDS * 16 <= row_bytes) && ((q & 15) == 0 || (r0 | k0) != 0)) {
+      const int have = n - r;
 #pragma unroll
-      for (int i = 0; i < kTileR; i += AT_ONCE, src += AT_ONCE * row_bytes)
-        if (i + AT_ONCE <= kTileR || i + r < kTileR)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + i * PITCH), "l"(src & ~(uintptr_t)15) : "memory");
+      for (int i = 0; i < ROWS; i += AT_ONCE, from += more)
+        if (i < have)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + i * PITCH), "l"(from & ~(uintptr_t)15) : "memory");
     } else {
 #pragma unroll 1
-      for (int i = r; i < kTileR && r0 + i < a.out; i += AT_ONCE, src += AT_ONCE * row_bytes, d += AT_ONCE * PITCH) {
-        const uintptr_t p = src & ~(uintptr_t)15;
-        const int64_t n = (int64_t)(reinterpret_cast<uintptr_t>(a.q) + (r0 + i + 1) * row_bytes) - (int64_t)p;  // to the row's end
-        if (p >= reinterpret_cast<uintptr_t>(a.q)) {
-          const uint32_t size = n >= 16 ? 16 : (n > 0 ? (uint32_t)n : 0);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(size ? p : reinterpret_cast<uintptr_t>(a.q)),
-                       "r"(size)
-                       : "memory");
+      for (int i = r; i < n; i += AT_ONCE, from += more, d += AT_ONCE * PITCH) {
+        const uintptr_t p = from & ~(uintptr_t)15;
+        const int64_t to_end = (int64_t)(q + (uint64_t)(r0 + i + 1) * row_bytes) - (int64_t)p;  // of the row
+        if (p >= q) {
+          const uint32_t size = to_end >= 16 ? 16 : (to_end > 0 ? (uint32_t)to_end : 0);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(size ? p : q & ~(uintptr_t)15), "r"(size) : "memory");
         } else {
-          uint8_t* const e = st + i * PITCH + w * 16;
+          uint8_t* const e = st + i * PITCH + lane % WORDS * 16;
 #pragma unroll 1
-          for (int b = 0; b < 16; b++)
-            e[b] = b < n && p + b >= reinterpret_cast<uintptr_t>(a.q) ? *reinterpret_cast<const uint8_t*>(p + b) : 0;
+          for (int b = 0; b < 16; b++) e[b] = b < to_end && p + b >= q ? *reinterpret_cast<const uint8_t*>(p + b) : 0;
         }
       }
     }
   }
 };
 
-// Tables in shared memory: a code byte as its two weights in bfloat16, one
-// copy per lane so that no two lanes meet in a bank (entry b of lane l at 128
-// b + 4 l), and a block's scale byte as a bfloat16 pair.  Per pair of weights
-// that leaves a byte extraction, an address, one load and the multiplication
-// by the scale, spread over four pipes; with integer operations alone (5 per
-// pair on the half-rate pipe) 8 rows x 8192^2 took 32 us.
-constexpr int kTableBytes = 256 * 128 + 256 * 4;
-template <int KIND>
+// Weights come from tables in shared memory or by byte permutes.  Tables: a
+// code byte as its two weights in bfloat16 and a block's scale byte as a
+// bfloat16 pair, one copy per lane so that no two lanes meet in a bank: entry
+// b of lane l at 256 b + 4 l, scales 128 further on.  With that stride one
+// byte permute puts a byte and the lane together as an address, so a pair of
+// weights takes a permute, a load and the multiplication by the scale.
+// Without them only the scales have a table, of one copy, and a pair takes
+// four permutes and logical operations and the multiplication.  With tables
+// the bound is shared memory's one access a cycle (8 rows x 8192^2: 15.8
+// accesses a warp for 16 weights of a lane, half of them look-ups), without
+// them the integer pipes: 20.5 us against 21.7, one row x 4096^2 6.6 against
+// 7.4, the backward product of 4 float32 rows x 4096^2 13.4 against 14.8.
+// From 16 columns of the mma on there is no room for two CTAs' tables (one
+// CTA of 16 rows x 8192^2 with them took 32.5 us, two without 26.3).
+template <bool TABLES>
+constexpr int kTableBytes = TABLES ? 256 * 256 : 256 * 4;
+template <int KIND, bool TABLES>
 __device__ __forceinline__ void make_tables(uint8_t* table) {
   static_assert(kRowThreads == 256, "a thread per entry");
   const int e = threadIdx.x;
-  const uint32_t pair = __byte_perm(__float_as_uint(W4<KIND>::value(e >> 4, 1.0f)),
-                                    __float_as_uint(W4<KIND>::value(e & 15, 1.0f)), 0x7632);
-  uint4* d = reinterpret_cast<uint4*>(table + e * 128);
+  const uint32_t scale = w4_scale_bf16x2<KIND>(e);
+  if (!TABLES) {
+    reinterpret_cast<uint32_t*>(table)[e] = scale;
+    return;
+  }
+  uint32_t raw[4];
+  w4_raw8<KIND>(e, raw);
+  const uint32_t pair = mul_bf16x2(raw[0], kTwo126);
+  uint4* d = reinterpret_cast<uint4*>(table + e * 256);
 #pragma unroll
-  for (int i = 0; i < 8; i++) d[(i + e) & 7] = make_uint4(pair, pair, pair, pair);  // turned, so that lanes differ in bank
-  reinterpret_cast<uint32_t*>(table + 256 * 128)[e] = w4_scale_bf16x2<KIND>(e);
+  for (int i = 0; i < (KIND == Q_MXFP4 ? 8 : 16); i++) {  // E8M0's scales without zero and NaN take no table
+    const uint32_t v = i < 8 ? pair : scale;
+    d[(i & 8) | ((i + e) & 7)] = make_uint4(v, v, v, v);  // turned, so that lanes differ in bank
+  }
 }
 
 // word at a byte offset of shared memory (a multiple of four)
@@ -135,22 +159,53 @@ struct At16 {
 __device__ __forceinline__ At16 at16(uint32_t block, uint32_t half) {
   return {(block + half) & ~3u, (block + half) * 8, block + 16};
 }
+// byte i of w as the place of this lane's table entry; lane4: four times the lane's number
+__device__ __forceinline__ uint32_t entry(uint32_t w, int i, uint32_t lane4) { return __byte_perm(w, lane4, 0x5504 + 16 * i); }
 // their two code words and scale (as a bfloat16 pair), `ahead` bytes further on
-template <int KIND>
-__device__ __forceinline__ void load16(const uint8_t* sm, const At16& at, uint32_t ahead, uint32_t w[2], uint32_t& f) {
+template <int KIND, bool TABLES>
+__device__ __forceinline__ void load16(const uint8_t* sm, const At16& at, uint32_t ahead, uint32_t lane4, uint32_t w[2],
+                                       uint32_t& f) {
   const uint32_t v0 = word(sm, at.word + ahead), v1 = word(sm, at.word + ahead + 4), v2 = word(sm, at.word + ahead + 8);
-  const uint32_t sb = W4<KIND>::MX ? sm[at.scale + ahead] : shift_down(v2, 0, at.shift) & 0xffu;
+  const uint32_t sb = W4<KIND>::MX ? sm[at.scale + ahead] : shift_down(v2, 0, at.shift);  // in the lowest byte
   w[0] = shift_down(v0, v1, at.shift), w[1] = shift_down(v1, v2, at.shift);
-  f = word(sm, 256 * 128 + sb * 4);
+  if (KIND == Q_MXFP4)
+    f = sb * 0x00800080u;  // the byte is a bfloat16's exponent
+  else
+    f = word(sm, TABLES ? entry(sb, 0, lane4) + 128 : (sb & 0xffu) * 4);
 }
-// the sixteen weights of two code words, o[i] = weights 2 i and 2 i + 1;
-// lane4: four times this lane's number
+// the eight weights of a code word, o[i] = weights 2 i and 2 i + 1: from the table
+__device__ __forceinline__ void look_up(const uint8_t* sm, uint32_t lane4, uint32_t w, uint32_t f, uint32_t o[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) o[i] = mul_bf16x2(word(sm, entry(w, i, lane4)), f);
+}
+// and by byte permutes alone: a permute looks four magnitudes' high bytes up
+// in eight, one their low bytes, and one spreads their signs (a selector's
+// highest bit repeats the sign of the byte, 0x80, so 0x80 or 0xff)
+template <int KIND>
+__device__ __forceinline__ void permute(uint32_t w, uint32_t f, uint32_t o[4]) {
+  constexpr uint32_t half = KIND == Q_MXFP4_OCP ? 0x3f00u : 0u;  // code 1
+  const uint32_t mag = w & 0x77777777u;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const uint32_t hi = __byte_perm(0x3f3f0000u | half, 0x40404040u, mag >> 16 * i);
+    const uint32_t lo = __byte_perm(0xc0800000u, 0xc0804000u, mag >> 16 * i);
+    uint32_t sg;
+    asm("prmt.b32 %0, %1, %1, %2;" : "=r"(sg) : "r"(0x80808080u), "r"(w >> 16 * i));
+    const uint32_t h = hi | (sg << 1 & 0x80808080u);
+    o[2 * i] = mul_bf16x2(__byte_perm(lo, h, 0x4051), f);
+    o[2 * i + 1] = mul_bf16x2(__byte_perm(lo, h, 0x6273), f);
+  }
+}
+// the sixteen of two
+template <int KIND, bool TABLES>
 __device__ __forceinline__ void decode16(const uint8_t* sm, uint32_t lane4, uint32_t w0, uint32_t w1, uint32_t f,
                                          uint32_t o[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const uint32_t b = __byte_perm(i < 4 ? w0 : w1, 0, 0x4440 + (i & 3));
-    o[i] = mul_bf16x2(word(sm, b * 128 + lane4), f);
+  if (TABLES) {
+    look_up(sm, lane4, w0, f, o);
+    look_up(sm, lane4, w1, f, o + 4);
+  } else {
+    permute<KIND>(w0, f, o);
+    permute<KIND>(w1, f, o + 4);
   }
 }
 
@@ -237,26 +292,24 @@ struct Column {
   }
 };
 
-// Adds what `n` floats of WARPS warps (at red + warp * n) and every CTA of the
+// Adds what `n` floats of the eight warps (at red + warp * n) and every CTA of the
 // cluster hold, always in the same order, and stores `count` results: result
 // o is the sum of the `parts` sums at place(o), place(o) + step, ...
-template <int WARPS, class Place, class Store>
+template <class Place, class Store>
 __device__ __forceinline__ void add_and_store(float* red, int n, int count, int parts, int step, Place&& place,
                                               Store&& store) {
   const uint32_t ranks = cluster_size(), rank = cluster_rank();
   __syncthreads();
-  if (WARPS > 1) {
 #pragma unroll 1
-    for (int i = threadIdx.x; i < n; i += kRowThreads) {
-      float v[WARPS];
+  for (int i = threadIdx.x; i < n; i += kRowThreads) {
+    float v[kRowWarps];
 #pragma unroll
-      for (int w = 0; w < WARPS; w++) v[w] = red[w * n + i];
+    for (int w = 0; w < kRowWarps; w++) v[w] = red[w * n + i];
 #pragma unroll
-      for (int w = 1; w < WARPS; w++) v[0] = __fadd_rn(v[0], v[w]);
-      red[i] = v[0];
-    }
-    __syncthreads();
+    for (int w = 1; w < kRowWarps; w++) v[0] = __fadd_rn(v[0], v[w]);
+    red[i] = v[0];
   }
+  __syncthreads();
   if (ranks > 1) cluster_barrier();
 #pragma unroll 1
   for (int o = rank * kRowThreads + threadIdx.x; o < count; o += ranks * kRowThreads) {
@@ -280,106 +333,125 @@ __device__ __forceinline__ void add_and_store(float* red, int n, int count, int 
   if (ranks > 1) cluster_barrier();  // nobody leaves while its sums are being read
 }
 
-// y[m, n]: a CTA (or cluster) takes 16 weight rows n at a time, every
-// gridDim.x / cluster-th such tile; NT * 8 columns of the mma hold rows x
-// parts.  The weight's bytes of the next tile are under way while a tile's
-// sums are added.
+// y[m, n]: two CTAs of eight warps per SM, of which one computes while the
+// other adds.  Each CTA, or cluster where there are few weight rows, takes a
+// run of weight rows n, cut at multiples of eight so that all have about the
+// same number, and goes through it 16 at a time; a warp goes through 256
+// columns of them at a time, and the next tiles' bytes are under way while a
+// tile's sums are added.  NT * 8 columns of the mma hold rows x parts; their x
+// comes from L1 and L2, AHEAD times 64 columns before it is used (32 rows x
+// 8192^2: 34 us with one and 46 us with two, which spills; 8 rows 20.8 us with
+// two, 22.0 with one).  One CTA of 16 warps and 32 weight rows that share x
+// took as long for 8 rows and 7.1 instead of 6.6 us for one row x 4096^2.
 template <int NT>
-constexpr int kForwardDepth = NT == 4 ? 2 : 3;  // two CTAs per SM
+struct Forward {
+  static constexpr bool TABLES = NT == 1;
+  static constexpr int AHEAD = NT <= 2 ? 2 : 1;
+  static constexpr int DEPTH = NT == 1 ? 2 : 3;      // tiles in a warp's ring
+  static constexpr int SUMS = kTileR * (NT * 8 + 1);  // [weight row][column], an odd pitch
+};
 template <int KIND, int DT, int NT>
 __global__ void __launch_bounds__(kRowThreads, 2) rows_forward_kernel(const RowArgs a) {
   using W = W4<KIND>;
-  using R = Ring<KIND, 256>;
-  constexpr int P = bf16_parts(DT), C = NT * 8, kDepth = kForwardDepth<NT>;
+  using S = Forward<NT>;
+  using R = Ring<KIND, 256, kTileR>;
+  constexpr int P = bf16_parts(DT), C = NT * 8, D = S::DEPTH;
   extern __shared__ __align__(16) uint8_t sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* const ring = sm + kTableBytes + warp * kDepth * R::BYTES;
-  float* const red = reinterpret_cast<float*>(sm + kTableBytes + kRowWarps * kDepth * R::BYTES);
-  const int in = (int)a.in, steps = (in + 255) / 256, stride = kRowWarps * (int)cluster_size();
+  uint8_t* const ring = sm + kTableBytes<S::TABLES> + warp * D * R::BYTES;
+  float* const red = reinterpret_cast<float*>(sm + kTableBytes<S::TABLES> + kRowWarps * D * R::BYTES);
+  const int in = (int)a.in, out = (int)a.out, steps = (in + 255) / 256, stride = kRowWarps << a.cluster;
   const int me = (int)cluster_rank() * kRowWarps + warp;
-  const int mine = me < steps ? (steps - me + stride - 1) / stride : 0;  // this warp's steps of a tile
-  const int64_t tiles = (a.out + kTileR - 1) / kTileR, tile_stride = gridDim.x / cluster_size();
-  int64_t tile = blockIdx.x / cluster_size();
-  make_tables<KIND>(sm);
-  const uint32_t lane4 = lane * 4, at0 = kTableBytes + warp * kDepth * R::BYTES + g * R::PITCH + 16 * t / W::BE * W::SB;
-  const uint32_t half = 16 * t % W::BE / 2;  // this lane's 16 of every 64 columns: a block, or half a block of 32
+  const int mine = (steps - me + stride - 1) >> (a.cluster + 3);  // this warp's steps of a piece (me < stride)
+  const int run = blockIdx.x >> a.cluster;
+  const int first = 8 * (run * a.per + min(run, a.extra)), last = min(out, first + 8 * (a.per + (run < a.extra)));
   const uint32_t q0 = (uint32_t)reinterpret_cast<uintptr_t>(a.q), row_bytes = (uint32_t)(a.in / W::BE * W::SB);
+  constexpr uint32_t STEP = 256 / W::BE * W::SB;
+  // what is fetched next: step fs (of `mine`) of the rows from fr
+  uintptr_t from = R::place(a, first, lane);
+  int fr = first, fs = 0, slot = 0;
+  const auto fetch = [&](int to) {
+    const int s = me + fs * stride;
+    if (fs < mine && fr < last)
+      R::fetch(a, ring + to * R::BYTES, from, fr, min(last - fr, kTileR), s * 256, s * STEP, lane);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++fs >= mine) fs = 0, fr += kTileR, from += (uint64_t)row_bytes * kTileR;
+  };
+#pragma unroll 1
+  for (int i = 0; i < D - 1; i++) fetch(i);
+  make_tables<KIND, S::TABLES>(sm);
+  const uint32_t lane4 = lane * 4, at0 = kTableBytes<S::TABLES> + warp * D * R::BYTES + g * R::PITCH + 16 * t / W::BE * W::SB;
+  const uint32_t half = 16 * t % W::BE / 2;  // this lane's 16 of every 64 columns: a block, or half a block of 32
   const float scale = out_scale(a.o);
   Column<DT> cols[NT];
 #pragma unroll
   for (int n = 0; n < NT; n++) cols[n].set(a, n * 8 + g);
-  // what is fetched next: step fs (of `mine`) of tile ft
-  int64_t ft = tile;
-  int fs = 0, slot = 0;
-  const auto fetch = [&](int to) {
-    if (fs < mine && ft < tiles) R::fetch(a, ring + to * R::BYTES, ft * kTileR, (me + fs * stride) * 256, lane);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    if (++fs >= mine) fs = 0, ft += tile_stride;
-  };
-#pragma unroll 1
-  for (int i = 0; i < kDepth - 1; i++) fetch(i);
-  // the next run's 16 elements of the columns' rows (zeros behind the rows' end)
-  uint32_t x[2][NT][8];
+  // the columns' rows, AHEAD times 64 columns (zeros behind the rows' end)
+  uint32_t x[S::AHEAD][NT][8];
   const auto load_x = [&](int k, uint32_t (*o)[8]) {
     const bool all = a.wide && k + 16 <= in;
 #pragma unroll
     for (int n = 0; n < NT; n++) cols[n].load16(k, in, all, o[n]);
   };
-  load_x(me * 256 + 16 * t, x[0]);
+#pragma unroll
+  for (int h = 0; h < S::AHEAD; h++) load_x(me * 256 + 16 * t + 64 * h, x[h]);
   __syncthreads();
 #pragma unroll 1
-  for (; tile < tiles; tile += tile_stride) {
-    const int64_t r0 = tile * kTileR;
-    const uint32_t sk0 = q0 + (uint32_t)(r0 + g) * row_bytes, sk1 = sk0 + 8 * row_bytes;
-    float acc[NT][4] = {}, part[NT][4] = {};  // part: of two steps, 32 mma (a tensor core cuts low bits off)
+  for (int r0 = first; r0 < last; r0 += kTileR) {
+    float acc[NT][4] = {};
 #pragma unroll 1
     for (int i = 0; i < mine; i++) {
       const int s = me + i * stride, k0 = s * 256 + 16 * t;
       const int next = i + 1 < mine ? k0 + stride * 256 : me * 256 + 16 * t;  // where the step after this one begins
       __syncwarp();  // all lanes are done with the stage that is filled next
-      fetch(slot == 0 ? kDepth - 1 : slot - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      fetch(slot == 0 ? D - 1 : slot - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
       __syncwarp();
-      const uint32_t adv = (uint32_t)s * (256 / W::BE * W::SB), off = at0 + slot * R::BYTES;
-      slot = slot + 1 == kDepth ? 0 : slot + 1;
+      const uint32_t sk = q0 + (uint32_t)(r0 + g) * row_bytes + (uint32_t)s * STEP;
+      const uint32_t off = at0 + slot * R::BYTES;
+      slot = slot + 1 == D ? 0 : slot + 1;
       // 64 columns are 34 or 36 bytes, 128 a multiple of four: two places a row
       constexpr uint32_t RUN = 64 / W::BE * W::SB;
-      const uint32_t p0 = off + ((sk0 + adv) & 15u), p1 = off + 8 * R::PITCH + ((sk1 + adv) & 15u);
+      const uint32_t p0 = off + (sk & 15u), p1 = off + 8 * R::PITCH + ((sk + 8 * row_bytes) & 15u);
       const At16 e0[2] = {at16(p0, half), at16(p0 + RUN, half)}, e1[2] = {at16(p1, half), at16(p1 + RUN, half)};
+      float part[NT][4] = {};  // 16 mma (a tensor core cuts low bits off)
 #pragma unroll 1
-      for (int b = 0; b < 2; b++)
+      for (int b = 0; b < 4; b += S::AHEAD)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          load_x(b + h < 2 ? k0 + 128 * b + 64 * h + 64 : next, x[1 - h]);
+        for (int h = 0; h < S::AHEAD; h++) {
+          const int run = b + h;
           uint32_t w0[2], w1[2], f0, f1, o0[8], o1[8];
-          load16<KIND>(sm, e0[h], 2 * RUN * b, w0, f0);
-          load16<KIND>(sm, e1[h], 2 * RUN * b, w1, f1);
-          decode16(sm, lane4, w0[0], w0[1], f0, o0);
-          decode16(sm, lane4, w1[0], w1[1], f1, o1);
+          if (S::AHEAD == 1) {
+            load16<KIND, S::TABLES>(sm, at16(p0 + RUN * run, half), 0, lane4, w0, f0);
+            load16<KIND, S::TABLES>(sm, at16(p1 + RUN * run, half), 0, lane4, w1, f1);
+          } else {
+            load16<KIND, S::TABLES>(sm, e0[h & 1], RUN * (run - (h & 1)), lane4, w0, f0);
+            load16<KIND, S::TABLES>(sm, e1[h & 1], RUN * (run - (h & 1)), lane4, w1, f1);
+          }
+          decode16<KIND, S::TABLES>(sm, lane4, w0[0], w0[1], f0, o0);
+          decode16<KIND, S::TABLES>(sm, lane4, w1[0], w1[1], f1, o1);
 #pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int j = 0; j < 8; j += 2)
               mma16816(part[n], o0[j], o1[j], o0[j + 1], o1[j + 1], x[h][n][j], x[h][n][j + 1]);
+          load_x(run + S::AHEAD < 4 ? k0 + 64 * (run + S::AHEAD) : next + 64 * (run + S::AHEAD - 4), x[h]);
         }
-      if ((i & 1) || i + 1 == mine) {
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+      for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) acc[n][j] = __fadd_rn(acc[n][j], part[n][j]), part[n][j] = 0.0f;
-      }
+        for (int j = 0; j < 4; j++) acc[n][j] = __fadd_rn(acc[n][j], part[n][j]);
     }
-    // red: [warp][weight row][column], an odd pitch
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-      float* d = red + warp * kTileR * (C + 1) + n * 8 + 2 * t;
-      d[g * (C + 1)] = acc[n][0], d[g * (C + 1) + 1] = acc[n][1];
-      d[(g + 8) * (C + 1)] = acc[n][2], d[(g + 8) * (C + 1) + 1] = acc[n][3];
+      float* const d = red + warp * S::SUMS + g * (C + 1) + n * 8 + 2 * t;
+      d[0] = acc[n][0], d[1] = acc[n][1];
+      d[8 * (C + 1)] = acc[n][2], d[8 * (C + 1) + 1] = acc[n][3];
     }
-    add_and_store<kRowWarps>(
-        red, kTileR * (C + 1), kTileR * a.rows, P, 1, [&](int o) { return (o & 15) * (C + 1) + (o >> 4) * P; },
+    add_and_store(
+        red, S::SUMS, kTileR * a.rows, P, 1, [&](int o) { return o % kTileR * (C + 1) + o / kTileR * P; },
         [&](int o, float v) {
-          if (r0 + (o & 15) < a.out) finish(a.o, scale, o >> 4, r0 + (o & 15), v);
+          if (o % kTileR < last - r0) finish(a.o, scale, o / kTileR, (int64_t)r0 + o % kTileR, v);
         });
     __syncthreads();  // red is free again
   }
@@ -391,17 +463,17 @@ constexpr int kDK = 128, kRedPitch = kDK + 8;  // a column's sums: 17 floats per
 template <int KIND, int DT, int NT>
 __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArgs a) {
   using W = W4<KIND>;
-  using R = Ring<KIND, kDK>;
+  using R = Ring<KIND, kDK, kTileR>;
   constexpr int P = bf16_parts(DT), C = NT * 8;
   extern __shared__ __align__(16) uint8_t sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t k0 = (int64_t)(blockIdx.x / cluster_size()) * kDK;
   const int64_t steps = (a.out + kTileR - 1) / kTileR, stride = (int64_t)kRowWarps * cluster_size();
-  uint8_t* const ring = sm + kTableBytes + warp * kDepth * R::BYTES;
+  uint8_t* const ring = sm + kTableBytes<true> + warp * kDepth * R::BYTES;
   // A warp's sums, [column][17 floats per 16 k].  Where it has more than 32
   // steps they have a place of their own and take the accumulators in every
   // 32 mma (a tensor core cuts low bits off); else they lie where the ring was.
-  float* const sums = reinterpret_cast<float*>(sm + (a.keep ? kTableBytes + kRowWarps * kDepth * R::BYTES : 0));
+  float* const sums = reinterpret_cast<float*>(sm + (a.keep ? kTableBytes<true> + kRowWarps * kDepth * R::BYTES : 0));
   int64_t ahead = (int64_t)cluster_rank() * kRowWarps + warp;
   uint32_t y[NT][2];  // of the next step
   Column<DT> cols[NT];
@@ -410,12 +482,12 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
     cols[n].set(a, n * 8 + g);
     cols[n].load(ahead * kTileR + 4 * t, a.out, a.wide, y[n]);
   }
-  make_tables<KIND>(sm);
+  make_tables<KIND, true>(sm);
   __syncthreads();
   const uint32_t q0 = (uint32_t)reinterpret_cast<uintptr_t>(a.q), row_bytes = (uint32_t)(a.in / W::BE * W::SB);
   const uint32_t sk = q0 + (uint32_t)(k0 / W::BE) * W::SB;
   // this lane's 16 columns: a block, or half a block of 32
-  const uint32_t at0 = kTableBytes + warp * kDepth * R::BYTES + 16 * g / W::BE * W::SB, half = 16 * g % W::BE / 2;
+  const uint32_t at0 = kTableBytes<true> + warp * kDepth * R::BYTES + 16 * g / W::BE * W::SB, half = 16 * g % W::BE / 2;
   int slot = 0;
   int64_t s = ahead - (kDepth - 1) * stride;
   bool first = true;
@@ -426,7 +498,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
 #pragma unroll 1
     for (; s < end; s += stride, ahead += stride, slot = slot + 1 == kDepth ? 0 : slot + 1) {
       __syncwarp();  // all lanes are done with the stage that is filled next
-      if (ahead < steps) R::fetch(a, ring + slot * R::BYTES, ahead * kTileR, (int)k0, lane);
+      if (ahead < steps) R::fetch(a, ring + slot * R::BYTES, R::place(a, ahead * kTileR, lane), (int)ahead * kTileR, min(kTileR, (int)a.out - (int)ahead * kTileR), (int)k0, (int)k0 / W::BE * W::SB, lane);
       asm volatile("cp.async.commit_group;" ::: "memory");
       if (s < 0) continue;
       uint32_t z[NT][2];
@@ -444,9 +516,9 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
       for (int r = 0; r < 4; r++) {
         const uint32_t block = st + (4 * t + r) * R::PITCH + ((sk + (uint32_t)(n0 + r) * row_bytes) & 15u);
         uint32_t w[2], f;
-        load16<KIND>(sm, at16(block, half), 0, w, f);
+        load16<KIND, true>(sm, at16(block, half), 0, lane * 4, w, f);
         if (n0 + r >= a.out) w[0] = w[1] = f = 0;  // behind the last row: whatever the stage held
-        decode16(sm, lane * 4, w[0], w[1], f, o[r]);
+        decode16<KIND, true>(sm, lane * 4, w[0], w[1], f, o[r]);
       }
 #pragma unroll
       for (int q = 0; q < 8; q++) {
@@ -472,7 +544,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
     first = false;
   } while (s < steps);
   const float scale = out_scale(a.o);
-  add_and_store<kRowWarps>(
+  add_and_store(
       sums, C * kRedPitch, kDK * a.rows, P, kRedPitch,
       [&](int o) { return (o >> 7) * P * kRedPitch + 17 * ((o & 127) >> 4) + (o & 15); },
       [&](int o, float v) {
@@ -485,16 +557,16 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
 // ---------------------------------------------------------------------------
 namespace {
 
-// CTAs that share a tile: two per SM are launched, and fewer tiles than that
-// are shared while every CTA still has a step for its warps
-int cluster_for(int64_t tiles, int64_t steps, int sms) {
+// CTAs that share a tile: `ctas` are launched at most, and fewer tiles than
+// that are shared while every CTA still has a step for its warps
+int cluster_for(int64_t tiles, int64_t steps, int ctas) {
   int cluster = 1;
-  while (cluster < 8 && tiles * cluster * 2 <= 2 * sms && cluster < steps) cluster *= 2;
+  while (cluster < 8 && tiles * cluster * 2 <= ctas && cluster < steps) cluster *= 2;
   return cluster;
 }
 
 template <void (*kernel)(const RowArgs)>
-cudaError_t launch_rows(const RowArgs& a, int64_t grid, int cluster, int smem, cudaStream_t st) {
+cudaError_t launch_rows(const RowArgs& a, int64_t tiles, int cluster, int smem, cudaStream_t st) {
   static int most[64] = {0};  // of this kernel, per device; setting it twice is harmless
   int dev = 0;
   cudaGetDevice(&dev);
@@ -504,11 +576,11 @@ cudaError_t launch_rows(const RowArgs& a, int64_t grid, int cluster, int smem, c
     if (dev >= 0 && dev < 64) most[dev] = smem;
   }
   if (cluster == 1) {
-    kernel<<<(unsigned)grid, kRowThreads, smem, st>>>(a);
+    kernel<<<(unsigned)tiles, kRowThreads, smem, st>>>(a);
     return cudaGetLastError();
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(grid * cluster));
+  cfg.gridDim = dim3((unsigned)(tiles * cluster));
   cfg.blockDim = dim3(kRowThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -521,18 +593,22 @@ cudaError_t launch_rows(const RowArgs& a, int64_t grid, int cluster, int smem, c
 
 template <int KIND, int DT, int NT>
 cudaError_t launch_one(const LinearArgs& l, RowArgs a, int sms, cudaStream_t st) {
-  const int64_t rows = (a.out + kTileR - 1) / kTileR;
   if (l.op == LIN_FORWARD) {
-    const int cluster = cluster_for(rows, (a.in + 256 * kRowWarps - 1) / (256 * kRowWarps), sms);
+    using S = Forward<NT>;
+    const int64_t units = (a.out + 7) / 8;
+    const int cluster = cluster_for(units, (a.in + 256 * kRowWarps - 1) / (256 * kRowWarps), 2 * sms);
+    const int64_t runs = std::min<int64_t>(units, 2 * sms / cluster);
+    while (1 << a.cluster < cluster) a.cluster++;
+    a.per = (int)(units / runs), a.extra = (int)(units % runs);
     return launch_rows<rows_forward_kernel<KIND, DT, NT>>(
-        a, std::min<int64_t>(rows, 2 * sms), cluster,
-        kTableBytes + kRowWarps * kForwardDepth<NT> * Ring<KIND, 256>::BYTES + kRowWarps * kTileR * (NT * 8 + 1) * 4, st);
+        a, runs, cluster,
+        kTableBytes<S::TABLES> + kRowWarps * (S::DEPTH * Ring<KIND, 256, kTileR>::BYTES + S::SUMS * 4), st);
   }
   if constexpr (NT <= 2) {
-    constexpr int ring = kTableBytes + kRowWarps * kDepth * Ring<KIND, kDK>::BYTES, sums = kRowWarps * NT * 8 * kRedPitch * 4;
-    const int64_t tiles = (a.in + kDK - 1) / kDK;
-    const int cluster = cluster_for(tiles, (rows + kRowWarps - 1) / kRowWarps, sms);
-    a.keep = rows > 32 * (int64_t)kRowWarps * cluster;
+    constexpr int ring = kTableBytes<true> + kRowWarps * kDepth * Ring<KIND, kDK, kTileR>::BYTES, sums = kRowWarps * NT * 8 * kRedPitch * 4;
+    const int64_t tiles = (a.in + kDK - 1) / kDK, steps = (a.out + kTileR - 1) / kTileR;
+    const int cluster = cluster_for(tiles, (steps + kRowWarps - 1) / kRowWarps, 2 * sms);
+    a.keep = steps > 32 * (int64_t)kRowWarps * cluster;
     return launch_rows<rows_dgrad_kernel<KIND, DT, NT>>(a, tiles, cluster, a.keep ? ring + sums : std::max(ring, sums), st);
   }
   return cudaErrorInvalidValue;
@@ -568,7 +644,7 @@ cudaError_t launch_few_rows(const LinearArgs& l, int sms, cudaStream_t st) {
   a.q = l.q;
   a.out = l.out, a.in = l.in;
   a.rows = (int)l.rows;
-  a.keep = 0;
+  a.keep = a.cluster = a.per = a.extra = 0;
   a.wide = (reinterpret_cast<uintptr_t>(l.a) & 15u) == 0 && (l.rows == 1 || (l.lda * (l.a_dtype == DT_F32 ? 4 : 2)) % 16 == 0);
   if (l.kind == Q_MXFP4) return launch_dt<Q_MXFP4>(l, a, sms, st);
   if (l.kind == Q_MXFP4_OCP) return launch_dt<Q_MXFP4_OCP>(l, a, sms, st);
