@@ -402,10 +402,12 @@ int ody_dequant_bf16(const void* q, int64_t n, float* out);   /* the exact BF16 
  * ody_get_quant and ody_quantize lay it out (blocks of the flattened tensor;
  * one may straddle two rows), any alignment.  x' is an activation kept in 8
  * bits (below).  Operands and results are float32, float16 or bfloat16, any
- * combination.  Every product is exact; sums are taken in float32 in an
- * order that depends on the shapes only (same call, same bits), and each
- * result is rounded once.  Non-finite inputs, and blocks with a non-finite
- * scale, make the results they reach non-finite.
+ * combination.  Every product is exact (float32 operands below 2^-109 lose
+ * their bits under 2^-133); sums are taken in float32 in an order that
+ * depends on the shapes only (same call, same bits), and each result is
+ * rounded once.  Non-finite inputs, and blocks with a non-finite scale, make
+ * the results they reach non-finite, though NaN may stand where the formula
+ * has an infinity.
  *
  * The plain forms take contiguous buffers in host or device memory and
  * return when done.  The _on_stream forms take memory of the current GPU

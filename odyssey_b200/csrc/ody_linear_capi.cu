@@ -68,12 +68,21 @@ int aligned_to(const void* p, int dtype, const char* what) {
   return ODY_OK;
 }
 
+// an error of the launcher itself is ours to report, not the next caller's to find
+int launched(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return ODY_OK;
+  cudaGetLastError();
+  return fail(ODY_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
 int launch(const LinearArgs& a, void* ws, cudaStream_t st) {
   if (aligned_to(a.a, a.a_dtype, "an operand") || aligned_to(a.o.c, a.o.dtype, "the output") ||
       (a.o.add && aligned_to(a.o.add, a.o.dtype, "add")))
     return ODY_ERR_ARG;
-  ODY_CUDA(launch_linear(a, ws, st));
-  return ODY_OK;
+  if (reinterpret_cast<uintptr_t>(a.o.tscale) % 4)
+    return fail(ODY_ERR_ARG, "the tensor scale is not aligned to its element type");
+  if (a.o.c == a.a || a.o.c == a.q) return fail(ODY_ERR_ARG, "the output must not be an operand");
+  return launched(launch_linear(a, ws, st), "launch_linear");
 }
 
 int on_stream(const LinearArgs& a, void* ws, size_t ws_bytes, void* stream, const char* name) {
@@ -162,8 +171,7 @@ extern "C" int ody_act8_save_on_stream(int32_t fmt, const void* x, int32_t dt, i
   return guarded([&]() -> int {
     if (int rc = act8_args(fmt, x, dt, rows, cols, ldx, codes, scales)) return rc;
     if (int rc = act8_device(x, dt, codes, scales, "ody_act8_save_on_stream")) return rc;
-    ODY_CUDA(launch_act8_save(fmt, x, dt, rows, cols, ldx, codes, scales, (cudaStream_t)stream));
-    return ODY_OK;
+    return launched(launch_act8_save(fmt, x, dt, rows, cols, ldx, codes, scales, (cudaStream_t)stream), "launch_act8_save");
   });
 }
 
@@ -172,8 +180,7 @@ extern "C" int ody_act8_load_on_stream(int32_t fmt, const uint8_t* codes, const 
   return guarded([&]() -> int {
     if (int rc = act8_args(fmt, out, dt, rows, cols, ldo, codes, scales)) return rc;
     if (int rc = act8_device(out, dt, codes, scales, "ody_act8_load_on_stream")) return rc;
-    ODY_CUDA(launch_act8_load(fmt, codes, scales, rows, cols, out, dt, ldo, (cudaStream_t)stream));
-    return ODY_OK;
+    return launched(launch_act8_load(fmt, codes, scales, rows, cols, out, dt, ldo, (cudaStream_t)stream), "launch_act8_load");
   });
 }
 
@@ -189,7 +196,8 @@ extern "C" int ody_act8_save(int32_t fmt, const void* x, int32_t dt, int64_t row
     ODY_STAGE(S, codes, (size_t)(rows * groups * kA8Group), false, &dc);
     ODY_STAGE(S, scales, (size_t)(rows * groups), false, &ds);
     if (int rc = act8_device(dx, dt, dc, ds, "ody_act8_save")) return rc;
-    ODY_CUDA(launch_act8_save(fmt, dx, dt, rows, cols, cols, (uint8_t*)dc, (uint8_t*)ds, S.st));
+    if (int rc = launched(launch_act8_save(fmt, dx, dt, rows, cols, cols, (uint8_t*)dc, (uint8_t*)ds, S.st), "launch_act8_save"))
+      return rc;
     ODY_CUDA(S.copy_out(codes));
     ODY_CUDA(S.copy_out(scales));
     ODY_CUDA(cudaStreamSynchronize(S.st));
@@ -209,7 +217,9 @@ extern "C" int ody_act8_load(int32_t fmt, const uint8_t* codes, const uint8_t* s
     ODY_STAGE(S, scales, (size_t)(rows * groups), true, &ds);
     ODY_STAGE(S, out, (size_t)(rows * cols) * dtype_size(dt), false, &dx);
     if (int rc = act8_device(dx, dt, dc, ds, "ody_act8_load")) return rc;
-    ODY_CUDA(launch_act8_load(fmt, (const uint8_t*)dc, (const uint8_t*)ds, rows, cols, dx, dt, cols, S.st));
+    if (int rc = launched(launch_act8_load(fmt, (const uint8_t*)dc, (const uint8_t*)ds, rows, cols, dx, dt, cols, S.st),
+                          "launch_act8_load"))
+      return rc;
     ODY_CUDA(S.copy_out(out));
     ODY_CUDA(cudaStreamSynchronize(S.st));
     return ODY_OK;

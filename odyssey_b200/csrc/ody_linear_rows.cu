@@ -240,7 +240,7 @@ struct Column {
   __device__ __forceinline__ void load16(int k, int n, bool all, uint32_t o[8]) const {
     if (all) {
       if (DT == DT_F32) {
-        const float4* s = reinterpret_cast<const float4*>(row + (uint32_t)k * 4);
+        const float4* s = reinterpret_cast<const float4*>(row + (uint64_t)(uint32_t)k * 4);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const float4 f = __ldg(s + i);

@@ -638,6 +638,9 @@ def test_refusals_on_device_memory(ody):
     assert call(x=host.ctypes.data) == L.ERR_ARG and call(y=host.ctypes.data) == L.ERR_ARG
     assert call(ts=host.ctypes.data) == L.ERR_ARG and call(ws=host.ctypes.data) == L.ERR_ARG
     assert call(x=x.data_ptr() + 2) == L.ERR_ARG and call(y=y.data_ptr() + 1) == L.ERR_ARG
+    scale = torch.ones(2, device="cuda")
+    assert call(ts=scale.data_ptr() + 2) == L.ERR_ARG
+    assert call(y=x.data_ptr()) == L.ERR_ARG and call(y=w.data.data_ptr()) == L.ERR_ARG
     torch.cuda.synchronize()
     assert (y == 5.0).all()
     assert call() == L.OK
@@ -676,6 +679,24 @@ def test_weight_of_more_than_2_32_elements(ody):
     d64 = R.to64(dy[:, rows])
     want = d64 @ w64
     R.check(ody.fp4_linear_dgrad(dy, w), want, R.tolerance(np.abs(d64) @ np.abs(w64), out, want, "float32"))
+
+
+def test_rows_of_more_than_2_32_bytes(ody):
+    """float32 features whose place in a row passes 32 bits: only the last 64
+    count (all other weights are zero), and the first 64 are large."""
+    inn, out = 2**30 + 64, 8
+    data = torch.zeros(out, inn // 32, 17, dtype=torch.uint8, device="cuda")
+    rng = np.random.default_rng(7)
+    last = rng.integers(0, 256, (out, 2, 17), dtype=np.uint8)
+    last[:, :, -1] = 127
+    data[:, -2:] = torch.from_numpy(last).cuda()
+    x = torch.zeros(1, inn, device="cuda")
+    x[0, :64] = 1e6
+    x[0, -64:] = torch.from_numpy(rng.standard_normal(64).astype(np.float32)).cuda()
+    w = ody.QuantizedTensor(data.view(-1), R.MXFP4, out * inn)
+    m = R.weight(R.MXFP4, last.reshape(-1), out, 64)
+    x64 = R.to64(x[:, -64:])
+    R.check(ody.fp4_linear(x, w), x64 @ m.T, R.tolerance(np.abs(x64) @ np.abs(m.T), 64, x64 @ m.T, "float32"))
 
 
 def test_activation_of_more_than_2_32_elements(ody):
