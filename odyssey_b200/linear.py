@@ -116,7 +116,7 @@ class _Place:
     """Where a buffer lies (what _same_place and _out ask of _Rows)."""
 
     def __init__(self, a):
-        self.a, self.cuda = a, L.is_torch(a) and a.is_cuda
+        self.a, self.cuda, self.code = a, L.is_torch(a) and a.is_cuda, None
 
 
 def _same_place(x, *others):
@@ -131,7 +131,7 @@ def _out(x, out, shape, code, what):
     """The result buffer: new, or the caller's after its checks."""
     if out is None:
         if L.is_torch(x.a):
-            return x.a.new_empty(shape, dtype=_torch_dtypes()[code])
+            return x.a.new_empty(shape) if code == x.code else x.a.new_empty(shape, dtype=_torch_dtypes()[code])
         return np.empty(shape, (np.float32, np.float16, np.uint16)[code])
     _same_place(x, out)
     have = _torch_dtypes().get(out.dtype) if L.is_torch(out) else \
@@ -148,15 +148,18 @@ def _flat(a):
     return a if a.is_contiguous() else a.contiguous()
 
 
-def _enqueue(index, call):
-    """call(stream) with that CUDA device current and torch's stream on it;
-    raises on a non-zero status."""
-    t = L._torch()
+def _enqueue(index, fn, *args):
+    """fn(*args, stream) with that CUDA device current and torch's stream on
+    it; raises on a non-zero status."""
+    t = L._torch_module
     if index != t.cuda.current_device():
         with t.cuda.device(index):
-            return L.check(call(t.cuda.current_stream(index).cuda_stream))
-    raw = getattr(t._C, "_cuda_getCurrentRawStream", None)  # the handle without a Stream object around it
-    return L.check(call(raw(index) if raw is not None else t.cuda.current_stream(index).cuda_stream))
+            rc = fn(*args, t.cuda.current_stream(index).cuda_stream)
+    else:
+        raw = getattr(t._C, "_cuda_getCurrentRawStream", None)  # the handle without a Stream object around it
+        rc = fn(*args, raw(index) if raw is not None else t.cuda.current_stream(index).cuda_stream)
+    if rc:
+        L.check(rc)
 
 
 @lru_cache(maxsize=4096)
@@ -164,32 +167,37 @@ def _workspace_bytes(device_index, op, rows, out, inn, code):
     return int(L.lib().ody_linear_workspace(op, rows, out, inn, code))
 
 
-def _workspace(a, op, rows, out, inn, code):
-    """(tensor or None, its address, its bytes) for one call on a's device."""
-    n = _workspace_bytes(a.get_device(), op, rows, out, inn, code)
+def _workspace(a, n):
+    """(tensor or None, its address, n) for one call on a's device."""
     if n <= 0:
         return None, None, 0
     ws = a.new_empty(n, dtype=L._torch().uint8)
     return ws, ws.data_ptr(), n
 
 
-def _product(name, op, x, w, out, out_dtype, dtype, what):
-    if not isinstance(w, QuantizedTensor) or w.kind not in _BLOCK:
-        raise L.OdysseyError(f"{name} takes a weight of the 4-bit kinds", L.ERR_ARG)
-    r = _Rows(x, dtype, what)
-    features, numel = r.cols, w.original_numel
+@lru_cache(maxsize=4096)
+def _weight(name, op, kind, numel, features):
+    """(the operand's other features, out features, in features, the weight's
+    bytes) of a weight of so many elements that meets so many features."""
     other = numel // features
     if numel <= 0 or other * features != numel:
         raise L.OdysseyError(f"{name}: a weight of {numel} elements has no rows of {features}" if op == L.LINEAR_FORWARD
                              else f"{name}: a weight of {numel} elements does not have {features} rows", L.ERR_SHAPE)
+    block, size = _BLOCK[kind]
     nout, nin = (other, features) if op == L.LINEAR_FORWARD else (features, other)
-    block, size = _BLOCK[w.kind]
-    need = (numel + block - 1) // block * size
+    return other, nout, nin, (numel + block - 1) // block * size
+
+
+def _product(name, op, x, w, out, out_dtype, dtype, what):
+    if not isinstance(w, QuantizedTensor) or w.kind not in _BLOCK:
+        raise L.OdysseyError(f"{name} takes a weight of the 4-bit kinds", L.ERR_ARG)
+    r = _Rows(x, dtype, what)
+    other, nout, nin, need = _weight(name, op, w.kind, w.original_numel, r.cols)
     data = w.data
     if L.numel(data) != need:
         raise L.OdysseyError(f"quantised buffer has {L.numel(data)} bytes, expected {need}", L.ERR_SHAPE)
     code = r.code if out_dtype is None else _code(out_dtype)
-    y = _out(r, out, r.lead + (other,), code, "out")
+    y = _out(r, out, (*r.lead, other), code, "out")
     lib = L.lib()
     _same_place(r, data)
     if not r.cuda:
@@ -207,10 +215,10 @@ def _product(name, op, x, w, out, out_dtype, dtype, what):
             ts = w.tensor_scale.data_ptr()
         else:
             alpha = w.tensor_scale
-    fn = lib.ody_fp4_linear_on_stream if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad_on_stream
-    ws, at, n = _workspace(r.a, op, r.rows, nout, nin, r.code)
-    _enqueue(r.a.get_device(), lambda st: fn(w.kind, data.data_ptr(), ts, alpha, nout, nin, r.ptr, r.code, r.rows, r.ld,
-                                       y.data_ptr(), code, other, at, n, st))
+    index = r.a.get_device()
+    ws, at, n = _workspace(r.a, _workspace_bytes(index, op, r.rows, nout, nin, r.code))
+    _enqueue(index, lib.ody_fp4_linear_on_stream if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad_on_stream, w.kind,
+             data.data_ptr(), ts, alpha, nout, nin, r.ptr, r.code, r.rows, r.ld, y.data_ptr(), code, other, at, n)
     return y
 
 
@@ -241,8 +249,8 @@ def save_activation8(x, format="e4m3", dtype=None):
         codes, scales = np.empty((r.rows, g * 32), np.uint8), np.empty((r.rows, g), np.uint8)
     lib = L.lib()
     if r.cuda:
-        _enqueue(r.a.get_device(), lambda st: lib.ody_act8_save_on_stream(fmt, r.ptr, r.code, r.rows, r.cols, r.ld,
-                                                                    codes.data_ptr(), scales.data_ptr(), st))
+        _enqueue(r.a.get_device(), lib.ody_act8_save_on_stream, fmt, r.ptr, r.code, r.rows, r.cols, r.ld,
+                 codes.data_ptr(), scales.data_ptr())
     else:
         L.check(lib.ody_act8_save(fmt, r.ptr, r.code, r.rows, r.cols, L.ptr(codes), L.ptr(scales)))
     return Activation8(codes, scales, r.rows, r.cols, format, r.lead + (r.cols,), _NAMES[r.code])
@@ -259,8 +267,8 @@ def load_activation8(a, dtype=None, out=None):
     y = _out(r, out, shape, code, "out")
     lib, fmt = L.lib(), FORMATS8[a.format]
     if r.cuda:
-        _enqueue(codes.get_device(), lambda st: lib.ody_act8_load_on_stream(fmt, codes.data_ptr(), scales.data_ptr(), a.rows,
-                                                                      a.cols, y.data_ptr(), code, a.cols, st))
+        _enqueue(codes.get_device(), lib.ody_act8_load_on_stream, fmt, codes.data_ptr(), scales.data_ptr(), a.rows, a.cols,
+                 y.data_ptr(), code, a.cols)
     else:
         L.check(lib.ody_act8_load(fmt, L.ptr(codes), L.ptr(scales), a.rows, a.cols, L.ptr(y), code))
     return y
@@ -289,11 +297,10 @@ def linear_wgrad8(dy, a, add=None, alpha=1.0, out=None, out_dtype=None, dtype=No
     codes, scales = L.contiguous(a.codes), L.contiguous(a.scales)
     fmt, lib = FORMATS8[a.format], L.lib()
     if r.cuda:
-        ws, at, n = _workspace(r.a, L.LINEAR_WGRAD, r.rows, r.cols, a.cols, r.code)
-        plus = None if add is None else add.data_ptr()
-        _enqueue(r.a.get_device(), lambda st: lib.ody_linear_wgrad8_on_stream(
-            fmt, codes.data_ptr(), scales.data_ptr(), a.rows, a.cols, r.ptr, r.code, r.cols, r.ld, alpha, plus,
-            y.data_ptr(), code, at, n, st))
+        index = r.a.get_device()
+        ws, at, n = _workspace(r.a, _workspace_bytes(index, L.LINEAR_WGRAD, r.rows, r.cols, a.cols, r.code))
+        _enqueue(index, lib.ody_linear_wgrad8_on_stream, fmt, codes.data_ptr(), scales.data_ptr(), a.rows, a.cols, r.ptr,
+                 r.code, r.cols, r.ld, alpha, None if add is None else add.data_ptr(), y.data_ptr(), code, at, n)
     else:
         L.check(lib.ody_linear_wgrad8(fmt, L.ptr(codes), L.ptr(scales), a.rows, a.cols, r.ptr, r.code, r.cols,
                                       C.c_float(alpha), None if add is None else L.ptr(add), L.ptr(y), code))
