@@ -19,8 +19,21 @@ __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.
 __device__ __forceinline__ void previous_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
-// Bringing operands to bfloat16
+// Bringing operands to bfloat16: one launch, whose first CTAs take the
+// quantised operand and whose others, if any, take x or dy.  (A launch each
+// cost 3 us more on the host, and on the GPU the smaller one's time.)
 // ---------------------------------------------------------------------------
+struct PrepareArgs {
+  const uint8_t* q;
+  const uint8_t* scales;  // wgrad
+  int64_t qrows, qcols, qp;
+  uint16_t* q16;  // [qrows, qp]
+  unsigned q_ctas;
+  const void* x;
+  int64_t rows, cols, ld, pitch, plane;
+  uint16_t* x16;  // planes of [rows, pitch]
+  int wide;       // x's rows are 16-byte aligned
+};
 
 // Rows of whole blocks: the weight is one flat run of blocks, so are its
 // bfloat16 values.  A tile of 8192 elements is 4608 or 4352 bytes, copied to
@@ -28,15 +41,13 @@ __device__ __forceinline__ void previous_done() { asm volatile("griddepcontrol.w
 // four times, so that neighbouring threads write neighbouring 16 bytes.
 constexpr int kUnpackTile = 8192;
 template <int KIND>
-__global__ void __launch_bounds__(256) unpack_w4_flat_kernel(const uint8_t* __restrict__ q, int64_t numel,
-                                                             uint16_t* __restrict__ out) {
+__device__ __forceinline__ void unpack_w4_flat(const PrepareArgs& p) {
   using W = W4<KIND>;
   constexpr int TB = kUnpackTile / W::BE * W::SB;
   __shared__ __align__(16) uint8_t sm[TB + 32];
-  let_next_start();
-  const int64_t t = blockIdx.x, b0 = t * TB, bytes = numel / W::BE * W::SB;
+  const int64_t t = blockIdx.x, numel = p.qrows * p.qcols, b0 = t * TB, bytes = numel / W::BE * W::SB;
   const int n = (int)(bytes - b0 < TB ? bytes - b0 : TB);
-  const uint8_t* src = q + b0;
+  const uint8_t* src = p.q + b0;
   const int skew = (int)(reinterpret_cast<uintptr_t>(src) & 15u);
   // 16-byte words that lie wholly inside the tile, single bytes around them
   const int head = skew ? 16 - skew : 0;
@@ -58,75 +69,64 @@ __global__ void __launch_bounds__(256) unpack_w4_flat_kernel(const uint8_t* __re
     w4_raw8<KIND>(w, o);
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = mul_bf16x2(mul_bf16x2(o[i], kTwo126), sc);
-    *reinterpret_cast<uint4*>(out + t * kUnpackTile + e) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(p.q16 + t * kUnpackTile + e) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
-// Any width: eight columns of a row per thread, the row padded to kp columns.
+// Any width: eight columns of a row per thread, the row padded to qp columns.
 template <int KIND>
-__global__ void __launch_bounds__(256) unpack_w4_rows_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols,
-                                                             int64_t kp, uint16_t* __restrict__ out) {
-  let_next_start();
-  const int64_t n = rows * (kp / 8), stride = (int64_t)gridDim.x * blockDim.x;
-  const bool blocks = cols % 8 == 0;  // eight columns share a block
-  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < n; t += stride) {
-    const int64_t r = t / (kp / 8), c = (t - r * (kp / 8)) * 8;
+__device__ __forceinline__ void unpack_w4_rows(const PrepareArgs& p) {
+  const int64_t n = p.qrows * (p.qp / 8), stride = (int64_t)p.q_ctas * 256;
+  const bool blocks = p.qcols % 8 == 0;  // eight columns share a block
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += stride) {
+    const int64_t r = t / (p.qp / 8), c = (t - r * (p.qp / 8)) * 8;
     EightQ<LIN_FORWARD, KIND> e;
-    e.load(q, nullptr, cols, r, c, (int)min((int64_t)8, cols - c), blocks);
-    e.store(reinterpret_cast<uint8_t*>(out + r * kp + c));
+    e.load(p.q, nullptr, p.qcols, r, c, (int)min((int64_t)8, p.qcols - c), blocks);
+    e.store(reinterpret_cast<uint8_t*>(p.q16 + r * p.qp + c));
   }
 }
 
 // 8-bit activations: eight columns per thread, rows of whole groups.
 template <int FMT>
-__global__ void __launch_bounds__(256) unpack_a8_kernel(const uint8_t* __restrict__ codes,
-                                                        const uint8_t* __restrict__ scales, int64_t n8,
-                                                        uint16_t* __restrict__ out) {
-  let_next_start();
-  const int64_t t0 = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+__device__ __forceinline__ void unpack_a8(const PrepareArgs& p) {
+  const int64_t t0 = (int64_t)blockIdx.x * 1024 + threadIdx.x, n8 = p.qrows * p.qp / 8;
   uint2 cs[4];
   uint32_t sbs[4];
 #pragma unroll
   for (int h = 0; h < 4; h++) {
     const int64_t t = min(t0 + h * 256, n8 - 1);
-    cs[h] = __ldcs(reinterpret_cast<const uint2*>(codes) + t);
-    sbs[h] = __ldg(scales + (t >> 2));
+    cs[h] = __ldcs(reinterpret_cast<const uint2*>(p.q) + t);
+    sbs[h] = __ldg(p.scales + (t >> 2));
   }
 #pragma unroll
   for (int h = 0; h < 4; h++) {
     const int64_t t = t0 + h * 256;
     if (t >= n8) return;
-    const uint2 c = cs[h];
-    const uint32_t sb = sbs[h];
     float v[8];
     uint32_t o[4];
-    a8_values8<FMT>(c, sb, v);
+    a8_values8<FMT>(cs[h], sbs[h], v);
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
-    reinterpret_cast<uint4*>(out)[t] = make_uint4(o[0], o[1], o[2], o[3]);
+    reinterpret_cast<uint4*>(p.q16)[t] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
-// x or dy as bf16_parts(DT) planes of [rows, cp] bfloat16, zeros behind cols.
+// x or dy as bf16_parts(DT) planes of [rows, pitch] bfloat16, zeros behind cols.
 template <int DT>
-__global__ void __launch_bounds__(256) pack_planes_kernel(const void* __restrict__ x, int64_t rows, int64_t cols,
-                                                          int64_t ldx, int64_t cp, int64_t plane, uint16_t* __restrict__ out,
-                                                          int wide) {
+__device__ __forceinline__ void pack_planes(const PrepareArgs& p) {
   constexpr int P = bf16_parts(DT);
-  let_next_start();
-  previous_done();
-  const int64_t n = rows * (cp / 8), stride = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < n; t += stride) {
-    const int64_t r = t / (cp / 8), c = (t - r * (cp / 8)) * 8, at = r * ldx + c;
+  const int64_t n = p.rows * (p.pitch / 8), stride = (int64_t)(gridDim.x - p.q_ctas) * 256;
+  for (int64_t t = (int64_t)(blockIdx.x - p.q_ctas) * 256 + threadIdx.x; t < n; t += stride) {
+    const int64_t r = t / (p.pitch / 8), c = (t - r * (p.pitch / 8)) * 8, at = r * p.ld + c;
     uint16_t h[8][3];
-    if (DT == DT_F32 && wide && c + 8 <= cols) {
-      const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + at);
+    if (DT == DT_F32 && p.wide && c + 8 <= p.cols) {
+      const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at);
       const float4 a = __ldg(s), b = __ldg(s + 1);
       const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
       for (int i = 0; i < 8; i++) split_bf16(v[i], h[i][0], h[i][1], h[i][2]);
-    } else if (DT != DT_F32 && wide && c + 8 <= cols) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + at));
+    } else if (DT != DT_F32 && p.wide && c + 8 <= p.cols) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at));
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int i = 0; i < 8; i++) {
@@ -139,14 +139,28 @@ __global__ void __launch_bounds__(256) pack_planes_kernel(const void* __restrict
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        split_bf16(c + i < cols ? load_elem(x, DT, at + i) : 0.0f, h[i][0], h[i][1], h[i][2]);
+        split_bf16(c + i < p.cols ? load_elem(p.x, DT, at + i) : 0.0f, h[i][0], h[i][1], h[i][2]);
     }
 #pragma unroll
-    for (int p = 0; p < P; p++)
-      *reinterpret_cast<uint4*>(out + p * plane + r * cp + c) =
-          make_uint4(h[0][p] | (uint32_t)h[1][p] << 16, h[2][p] | (uint32_t)h[3][p] << 16,
-                     h[4][p] | (uint32_t)h[5][p] << 16, h[6][p] | (uint32_t)h[7][p] << 16);
+    for (int k = 0; k < P; k++)
+      *reinterpret_cast<uint4*>(p.x16 + k * p.plane + r * p.pitch + c) =
+          make_uint4(h[0][k] | (uint32_t)h[1][k] << 16, h[2][k] | (uint32_t)h[3][k] << 16,
+                     h[4][k] | (uint32_t)h[5][k] << 16, h[6][k] | (uint32_t)h[7][k] << 16);
   }
+}
+
+enum : int { Q_FLAT, Q_ROWS, Q_ACT8 };  // how the quantised operand lies
+template <int HOW, int KIND, int DT>
+__global__ void __launch_bounds__(256) prepare_kernel(const PrepareArgs p) {
+  let_next_start();
+  if (blockIdx.x >= p.q_ctas)
+    pack_planes<DT>(p);
+  else if constexpr (HOW == Q_FLAT)
+    unpack_w4_flat<KIND>(p);
+  else if constexpr (HOW == Q_ROWS)
+    unpack_w4_rows<KIND>(p);
+  else
+    unpack_a8<KIND>(p);
 }
 
 // ---------------------------------------------------------------------------
@@ -757,17 +771,26 @@ cudaError_t launch_next(void (*kernel)(P...), dim3 grid, int threads, int smem, 
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
-template <int KIND>
-cudaError_t unpack_w4(const LinearArgs& a, const Plan& p, uint16_t* out, int sms, cudaStream_t st) {
-  if (a.in % W4<KIND>::BE == 0) {
-    const int64_t n = a.out * a.in;
-    unpack_w4_flat_kernel<KIND>
-        <<<(unsigned)((n + kUnpackTile - 1) / kUnpackTile), 256, 0, st>>>(a.q, n, out);
-  } else {
-    unpack_w4_rows_kernel<KIND>
-        <<<grid_for(p.qrows * p.qp / 8, sms), 256, 0, st>>>(a.q, p.qrows, p.qcols, p.qp, out);
-  }
+template <int HOW, int KIND>
+cudaError_t prepare(const PrepareArgs& p, int dtype, int x_ctas, cudaStream_t st) {
+  const unsigned grid = p.q_ctas + x_ctas;
+  if (dtype == DT_F32)
+    prepare_kernel<HOW, KIND, DT_F32><<<grid, 256, 0, st>>>(p);
+  else if (dtype == DT_F16)
+    prepare_kernel<HOW, KIND, DT_F16><<<grid, 256, 0, st>>>(p);
+  else
+    prepare_kernel<HOW, KIND, DT_BF16><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError();
+}
+
+template <int KIND>
+cudaError_t prepare_w4(PrepareArgs& p, int dtype, int x_ctas, int sms, cudaStream_t st) {
+  if (p.qcols % W4<KIND>::BE == 0) {
+    p.q_ctas = (unsigned)((p.qrows * p.qcols + kUnpackTile - 1) / kUnpackTile);
+    return prepare<Q_FLAT, KIND>(p, dtype, x_ctas, st);
+  }
+  p.q_ctas = grid_for(p.qrows * p.qp / 8, sms);
+  return prepare<Q_ROWS, KIND>(p, dtype, x_ctas, st);
 }
 
 template <bool AMN, bool BMN, int DT>
@@ -814,41 +837,33 @@ cudaError_t launch_gemm(const LinearArgs& a, void* ws, int sms, cudaStream_t st)
   const Plan p = make_plan(a, sms);
   uint8_t* base = static_cast<uint8_t*>(ws);
   uint16_t* q16 = reinterpret_cast<uint16_t*>(base + p.q_off);
-  cudaError_t e;
-  if (a.op == LIN_WGRAD) {
-    const int64_t n8 = p.qrows * p.qp / 8;
-    const unsigned grid = (unsigned)((n8 + 1023) / 1024);
-    if (a.kind == A8_E4M3)
-      unpack_a8_kernel<A8_E4M3><<<grid, 256, 0, st>>>(a.q, a.scales, n8, q16);
-    else
-      unpack_a8_kernel<A8_E5M2><<<grid, 256, 0, st>>>(a.q, a.scales, n8, q16);
-    e = cudaGetLastError();
-  } else if (a.kind == Q_MXFP4) {
-    e = unpack_w4<Q_MXFP4>(a, p, q16, sms, st);
-  } else if (a.kind == Q_MXFP4_OCP) {
-    e = unpack_w4<Q_MXFP4_OCP>(a, p, q16, sms, st);
-  } else {  // the tensor scale of ODY_Q_NVFP4_TENSOR is applied to the sums
-    e = unpack_w4<Q_NVFP4>(a, p, q16, sms, st);
-  }
-  if (e != cudaSuccess) return e;
+  PrepareArgs r{};
+  r.q = a.q, r.scales = a.scales, r.qrows = p.qrows, r.qcols = p.qcols, r.qp = p.qp, r.q16 = q16;
   // bfloat16 rows that TMA can read are used where they lie
   const void* abase = a.a;
   int64_t apitch = a.lda, aplane = a.lda;  // one plane: its pitch is never used
+  int x_ctas = 0;
   if (a.a_dtype != DT_BF16 || (reinterpret_cast<uintptr_t>(a.a) & 15u) || a.lda % 8) {
-    uint16_t* a16 = reinterpret_cast<uint16_t*>(base + p.a_off);
     const int64_t es = a.a_dtype == DT_F32 ? 4 : 2;
-    const int wide = (reinterpret_cast<uintptr_t>(a.a) & 15u) == 0 && (a.lda * es) % 16 == 0;
     apitch = p.ap, aplane = p.arows * p.ap;
-    const int grid = grid_for(p.arows * p.ap / 8, sms);
-    if (a.a_dtype == DT_F32)
-      e = launch_next(pack_planes_kernel<DT_F32>, grid, 256, 0, st, a.a, p.arows, p.acols, a.lda, apitch, aplane, a16, wide);
-    else if (a.a_dtype == DT_F16)
-      e = launch_next(pack_planes_kernel<DT_F16>, grid, 256, 0, st, a.a, p.arows, p.acols, a.lda, apitch, aplane, a16, wide);
-    else
-      e = launch_next(pack_planes_kernel<DT_BF16>, grid, 256, 0, st, a.a, p.arows, p.acols, a.lda, apitch, aplane, a16, wide);
-    if (e != cudaSuccess) return e;
-    abase = a16;
+    r.x = a.a, r.rows = p.arows, r.cols = p.acols, r.ld = a.lda, r.pitch = apitch, r.plane = aplane;
+    r.x16 = reinterpret_cast<uint16_t*>(base + p.a_off);
+    r.wide = (reinterpret_cast<uintptr_t>(a.a) & 15u) == 0 && (a.lda * es) % 16 == 0;
+    x_ctas = grid_for(p.arows * p.ap / 8, sms);
+    abase = r.x16;
   }
+  cudaError_t e;
+  if (a.op == LIN_WGRAD) {
+    r.q_ctas = (unsigned)((p.qrows * p.qp / 8 + 1023) / 1024);
+    e = a.kind == A8_E4M3 ? prepare<Q_ACT8, A8_E4M3>(r, a.a_dtype, x_ctas, st) : prepare<Q_ACT8, A8_E5M2>(r, a.a_dtype, x_ctas, st);
+  } else if (a.kind == Q_MXFP4) {
+    e = prepare_w4<Q_MXFP4>(r, a.a_dtype, x_ctas, sms, st);
+  } else if (a.kind == Q_MXFP4_OCP) {
+    e = prepare_w4<Q_MXFP4_OCP>(r, a.a_dtype, x_ctas, sms, st);
+  } else {  // the tensor scale of ODY_Q_NVFP4_TENSOR is applied to the sums
+    e = prepare_w4<Q_NVFP4>(r, a.a_dtype, x_ctas, sms, st);
+  }
+  if (e != cudaSuccess) return e;
   const bool amn = a.op == LIN_WGRAD, bmn = a.op != LIN_FORWARD;
   CUtensorMap ma, mb;
   if ((e = make_map(&ma, abase, p.acols, p.arows, p.planes, apitch, aplane, amn ? kBK : kHalf)) != cudaSuccess) return e;
