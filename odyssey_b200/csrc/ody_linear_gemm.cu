@@ -525,13 +525,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + half * (kBN / 2);
     const uint32_t done = in_cta(tempty, 0);
+    // a warp goes on, or stops after a wait that ran out, as one
+    const auto together = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
     float* buf32 = reinterpret_cast<float*>(dyn + (smem - sptr(dyn)) + kStages * kStageBytes) + (warp - 4) * 32 * 32;
     const float scale = out_scale(g.o);
     constexpr int ES = DT == DT_F32 ? 4 : 2;
     int chunk = 0;
     bool ok = true;
     Pieces w(g, pair);
-    while (ok && !*abort && w.get(g, pairs)) {
+    while (ok && together(!*abort) && w.get(g, pairs)) {
       int tm, tn;
       tile_at(g, w.tile, tm, tn);
       float acc[kBN / 2];
@@ -539,8 +541,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
       for (int i = 0; i < kBN / 2; i++) acc[i] = 0.0f;
       for (int c = w.s0; c < w.s1; c += g.chunk, chunk++) {
         const int buf = chunk & 1;
-        if (!(ok = mbar_wait(tfull + 8 * buf, (chunk / 2) & 1, abort))) break;
-        __syncwarp();
+        if (!(ok = together(mbar_wait(tfull + 8 * buf, (chunk / 2) & 1, abort)))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         // 32 columns are added while the next 32 are on their way
         uint32_t v[2][32];
