@@ -498,7 +498,11 @@ __global__ void __launch_bounds__(kRowThreads, 2) rows_dgrad_kernel(const RowArg
 #pragma unroll 1
     for (; s < end; s += stride, ahead += stride, slot = slot + 1 == kDepth ? 0 : slot + 1) {
       __syncwarp();  // all lanes are done with the stage that is filled next
-      if (ahead < steps) R::fetch(a, ring + slot * R::BYTES, R::place(a, ahead * kTileR, lane), (int)ahead * kTileR, min(kTileR, (int)a.out - (int)ahead * kTileR), (int)k0, (int)k0 / W::BE * W::SB, lane);
+      if (ahead < steps) {
+        const int r0 = (int)ahead * kTileR;
+        R::fetch(a, ring + slot * R::BYTES, R::place(a, r0, lane), r0, min(kTileR, (int)a.out - r0), (int)k0,
+                 (int)k0 / W::BE * W::SB, lane);
+      }
       asm volatile("cp.async.commit_group;" ::: "memory");
       if (s < 0) continue;
       uint32_t z[NT][2];
