@@ -284,10 +284,10 @@ static cudaError_t launch_medium_w4(const LinearArgs& a, const MediumPlan& p, cu
 // Which way a product goes: few rows of whole blocks in one pass over the
 // weight, medium ones in one launch, the others to the tcgen05 kernel after
 // their operands have been brought to bfloat16.  The medium kernel takes 4 us
-// and 0.9 us (float32 1.4) for each 64 of the reduction that an SM does; the
-// other's launches take 15 us (16 with an operand to be split): 512 x 1024 x
-// 1024 in bfloat16, 16 rounds, 17.4 us against 15.8; 256 x 1024 x 1024, 8
-// rounds, 10.3 against 15.7.
+// and about 1 us (float32 1.3) for each 64 of the reduction that an SM does,
+// the others start at 14 us (18 with an operand to be split).  512 x 1024 x
+// 1024, 16 rounds: 20.3 us against 15.3 in bfloat16, 25.6 against 19.1 in
+// float32; 256 x 1024 x 1024, 8 rounds: 12.0 against 14.4, 14.7 against 18.4.
 constexpr int64_t kMediumRounds = 12;
 static bool medium_product(const LinearArgs& a) { return medium_plan(a, lin_sms()).rounds <= kMediumRounds; }
 
