@@ -288,6 +288,12 @@ static cudaError_t launch_medium_w4(const LinearArgs& a, const MediumPlan& p, cu
 // the others start at 14 us (18 with an operand to be split).  512 x 1024 x
 // 1024, 16 rounds: 20.3 us against 15.3 in bfloat16, 25.6 against 19.1 in
 // float32; 256 x 1024 x 1024, 8 rounds: 12.0 against 14.4, 14.7 against 18.4.
+// The few-row kernels take all that their registers hold: 32 rows x 8192^2
+// forward 34 us, by the tcgen05 kernel 68; 16 rows backward 29 against 66; 5
+// rows x 1024^2 forward 3.8 us, by the medium kernel 7.4.  (Small products of
+// several float32 rows would gain there, 4 x 128 x 384 5.1 us for 7.9; they
+// stay, since among few rows a row's results then do not depend on how many
+// there are.)
 constexpr int64_t kMediumRounds = 12;
 static bool medium_product(const LinearArgs& a) { return medium_plan(a, lin_sms()).rounds <= kMediumRounds; }
 
