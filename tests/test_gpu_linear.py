@@ -472,6 +472,21 @@ def test_same_call_same_bits(ody):
                 assert torch.equal(f, s)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_do_not_depend_on_each_other(ody, dtype):
+    """Among few rows a row's results are the same bits whatever their number."""
+    rng = np.random.default_rng(21)
+    parts = {"bfloat16": 1, "float16": 2, "float32": 3}[dtype]
+    for out, inn in ((72, 1056), (600, 64), (1030, 2080)):
+        w, _ = make_w(ody, rng, "mxfp4", out, inn)
+        for fn, cols, most in ((ody.fp4_linear, inn, 32 // parts), (ody.fp4_linear_dgrad, out, 16 // parts)):
+            x = dev(rng.standard_normal((most, cols)).astype(np.float32), dtype)
+            whole = fn(x, w)
+            for n in (1, 2, 8 // parts, 8 // parts + 1):
+                assert torch.equal(fn(x[:n], w), whole[:n]), (out, inn, n)
+            assert torch.equal(fn(x[-1:], w), whole[-1:])
+
+
 def test_captured_and_replayed_on_side_streams(ody):
     """Two captured layers of different sizes, replayed at once on two streams
     with new inputs, give the bits of eager calls."""
