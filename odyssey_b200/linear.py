@@ -202,8 +202,8 @@ def _product(name, op, x, w, out, out_dtype, dtype, what):
     _same_place(r, data)
     if not r.cuda:
         fn = lib.ody_fp4_linear if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad
-        L.check(fn(w.kind, L.ptr(L.contiguous(data)), float(w.tensor_scale), nout, nin, r.ptr, r.code, r.rows, L.ptr(y),
-                   code))
+        data = L.contiguous(data)  # a copy of a strided buffer has to outlive the call
+        L.check(fn(w.kind, L.ptr(data), float(w.tensor_scale), nout, nin, r.ptr, r.code, r.rows, L.ptr(y), code))
         return y
     data = _flat(data)
     ts, alpha = None, 1.0

@@ -1,0 +1,55 @@
+"""What the quantised linear layer's Python calls hand to the library, and the
+buffers that they refuse, without a GPU."""
+import ctypes as C
+import types
+import weakref
+
+import numpy as np
+import pytest
+
+
+@pytest.fixture(scope="module")
+def ody():
+    from odyssey_b200.build import build
+    build()
+    import odyssey_b200
+    odyssey_b200.lib()
+    return odyssey_b200
+
+
+def refused(ody, code, match, fn, *args, **kw):
+    with pytest.raises(ody.OdysseyError, match=match) as e:
+        fn(*args, **kw)
+    assert e.value.code == code
+
+
+@pytest.mark.parametrize("name", ["fp4_linear", "fp4_linear_dgrad"])
+@pytest.mark.parametrize("torch_weight", [False, True])
+def test_strided_host_weight_lives_until_the_call_is_done(ody, monkeypatch, name, torch_weight):
+    """A weight that is not contiguous is copied; the copy is what the library
+    reads, so it is still there, with the weight's bytes, when it does."""
+    import torch
+    from odyssey_b200 import linear, _lib as L
+    out, inn = 512, 512
+    n = L.quant_bytes(L.Q_NVFP4, out * inn)
+    wide = np.random.default_rng(1).integers(0, 256, 2 * n, dtype=np.uint8)
+    want = wide[::2].tobytes()
+    data = torch.from_numpy(wide)[::2] if torch_weight else wide[::2]
+    copies, seen = [], []
+    contiguous = L.contiguous
+
+    def tracked(x):
+        c = contiguous(x)
+        copies.append(weakref.ref(c))
+        return c
+
+    def entry(kind, q, *rest):
+        decoys = [np.full(n, 0xEE, np.uint8) for _ in range(4)]  # what a freed copy's memory would be given to
+        seen.append((C.string_at(q, n) == want, [c() is not None for c in copies]))
+        return len(decoys) - 4
+
+    monkeypatch.setattr(linear.L, "contiguous", tracked)
+    monkeypatch.setattr(linear.L, "lib", lambda: types.SimpleNamespace(**{"ody_" + name: entry}))
+    w = ody.QuantizedTensor(data, L.Q_NVFP4, out * inn)
+    getattr(ody, name)(np.ones((2, 512), np.float32), w)
+    assert seen == [(True, [True])]
