@@ -19,6 +19,7 @@ dtype='bfloat16') are staged and the call returns when done.
 import ctypes as C
 from dataclasses import dataclass
 from functools import lru_cache
+from math import prod
 
 import numpy as np
 
@@ -261,6 +262,9 @@ def load_activation8(a, dtype=None, out=None):
     a.check()
     code = _code(dtype if dtype is not None else a.dtype if a.dtype is not None else L.BF16)
     shape = a.shape if a.shape is not None else (a.rows, a.cols)
+    if prod(shape) != a.rows * a.cols:
+        raise L.OdysseyError(f"the activation's shape {tuple(shape)} does not have the {a.rows * a.cols} elements of its rows "
+                             "and columns", L.ERR_SHAPE)
     codes, scales = L.contiguous(a.codes), L.contiguous(a.scales)
     r = _Place(codes)
     _same_place(r, scales)

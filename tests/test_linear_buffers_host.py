@@ -53,3 +53,15 @@ def test_strided_host_weight_lives_until_the_call_is_done(ody, monkeypatch, name
     w = ody.QuantizedTensor(data, L.Q_NVFP4, out * inn)
     getattr(ody, name)(np.ones((2, 512), np.float32), w)
     assert seen == [(True, [True])]
+
+
+def test_load_refuses_a_shape_of_other_elements(ody):
+    """The shape an Activation8 carries sizes the result, so it has to hold the
+    rows and columns that are written there: not fewer (a write past the
+    buffer), not more (an unwritten rest)."""
+    from odyssey_b200 import _lib as L
+    codes, scales = np.zeros((3, 64), np.uint8), np.zeros((3, 2), np.uint8)
+    for shape in ((2, 40), (3, 39), (40,), (), (0, 40), (4, 40), (3, 41), (2, 3, 40)):
+        a = ody.Activation8(codes, scales, 3, 40, shape=shape)
+        refused(ody, L.ERR_SHAPE, "120 elements", ody.load_activation8, a)
+        refused(ody, L.ERR_SHAPE, "120 elements", ody.load_activation8, a, out=np.empty(shape, np.float32), dtype="float32")
