@@ -98,9 +98,11 @@ struct Scope {
     *dev = d;
     return cudaSuccess;
   }
+  // Results are staged behind the operands, so of two entries of one address
+  // (an operand that is the result too) the later one holds the result.
   cudaError_t copy_out(void* user) {
-    for (auto& b : bufs)
-      if (b.user == user && b.owned) return cudaMemcpyAsync(user, b.dev, b.bytes, cudaMemcpyDeviceToHost, st);
+    for (auto b = bufs.rbegin(); b != bufs.rend(); ++b)
+      if (b->user == user && b->owned) return cudaMemcpyAsync(user, b->dev, b->bytes, cudaMemcpyDeviceToHost, st);
     return cudaSuccess;
   }
 };
