@@ -419,7 +419,9 @@ int ody_dequant_bf16(const void* q, int64_t n, float* out);   /* the exact BF16 
  * ody_linear_workspace(op, ...) bytes (may be 0).  tensor_scale (a device
  * float, or NULL for 1) is ODY_Q_NVFP4_TENSOR's; results are multiplied by
  * alpha * *tensor_scale.  Outputs must not overlap inputs, except that add
- * may be dw itself (accumulation in place). */
+ * may be dw itself (accumulation in place); columns of one wide buffer do not
+ * overlap.  Device buffers that share a byte, and host buffers of the same
+ * address, are refused (ODY_ERR_ARG). */
 #define ODY_LINEAR_FORWARD 0
 #define ODY_LINEAR_DGRAD 1
 #define ODY_LINEAR_WGRAD 2

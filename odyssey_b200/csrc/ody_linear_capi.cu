@@ -68,6 +68,45 @@ int aligned_to(const void* p, int dtype, const char* what) {
   return ODY_OK;
 }
 
+// A buffer as its rows: `n` of `bytes`, `pitch` bytes apart.
+struct Span {
+  const void* p;
+  int64_t n, bytes, pitch;
+};
+Span flat(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+
+// Whether two buffers share a byte.  Rows may interleave (columns of one wide
+// buffer), so where the extents meet, each row of the one with fewer rows is
+// compared with the first row of the other that ends behind its begin.
+bool meet(const Span& u, const Span& v) {
+  if (!u.p || !v.p) return false;
+  using Wide = __int128;  // a pitch times a number of rows may pass 64 bits
+  const Span &x = u.n <= v.n ? u : v, &y = u.n <= v.n ? v : u;
+  const Wide a = (Wide)(uintptr_t)x.p, b = (Wide)(uintptr_t)y.p;
+  const Wide a_end = a + (Wide)(x.n - 1) * x.pitch + x.bytes, b_end = b + (Wide)(y.n - 1) * y.pitch + y.bytes;
+  if (a_end <= b || b_end <= a) return false;
+  for (int64_t i = 0; i < x.n; i++) {
+    const Wide s = a + (Wide)i * x.pitch, e = s + x.bytes;
+    const Wide j = s - b < y.bytes ? 0 : (s - b - y.bytes) / y.pitch + 1;
+    if (j < y.n && b + j * y.pitch < e) return true;
+  }
+  return false;
+}
+
+constexpr const char* kOverlap = "the output must not be or overlap an operand";
+
+// the rows of a product's buffers
+struct Spans {
+  Span a, c, q, scales;
+  explicit Spans(const LinearArgs& l) {
+    const int64_t es = dtype_size(l.a_dtype), cs = dtype_size(l.o.dtype), groups = (l.in + kA8Group - 1) / kA8Group;
+    a = {l.a, l.rows, (l.op == LIN_FORWARD ? l.in : l.out) * es, l.lda * es};
+    c = {l.o.c, l.op == LIN_WGRAD ? l.out : l.rows, (l.op == LIN_FORWARD ? l.out : l.in) * cs, l.o.ld * cs};
+    q = flat(l.q, l.op == LIN_WGRAD ? l.rows * groups * kA8Group : ody_quant_bytes(l.kind, l.out * l.in));
+    scales = flat(l.scales, l.rows * groups);
+  }
+};
+
 // an error of the launcher itself is ours to report, not the next caller's to find
 int launched(cudaError_t e, const char* what) {
   if (e == cudaSuccess) return ODY_OK;
@@ -81,7 +120,10 @@ int launch(const LinearArgs& a, void* ws, cudaStream_t st) {
     return ODY_ERR_ARG;
   if (reinterpret_cast<uintptr_t>(a.o.tscale) % 4)
     return fail(ODY_ERR_ARG, "the tensor scale is not aligned to its element type");
-  if (a.o.c == a.a || a.o.c == a.q) return fail(ODY_ERR_ARG, "the output must not be an operand");
+  const Spans s(a);
+  const Span add = {a.o.add == a.o.c ? nullptr : a.o.add, s.c.n, s.c.bytes, s.c.pitch};
+  if (meet(s.c, s.a) || meet(s.c, s.q) || meet(s.c, s.scales) || meet(s.c, flat(a.o.tscale, 4)) || meet(s.c, add))
+    return fail(ODY_ERR_ARG, kOverlap);
   return launched(launch_linear(a, ws, st), "launch_linear");
 }
 
@@ -113,13 +155,13 @@ int status(cudaStream_t st) {
   return ran_out ? fail(ODY_ERR_DEVICE_BOUNDS, "a bounded wait inside a linear kernel ran out") : ODY_OK;
 }
 
-// host or device buffers, contiguous; waits for the result
+// Host or device buffers, contiguous; waits for the result.  (Host buffers
+// are copied, so the output's copy never meets another one: the caller's own
+// addresses are compared first.)
 int staged(LinearArgs a, float alpha) {
-  const int64_t asz = a.rows * a.lda * (int64_t)dtype_size(a.a_dtype);
-  const int64_t crows = a.op == LIN_WGRAD ? a.out : a.rows;
-  const int64_t csz = crows * a.o.ld * (int64_t)dtype_size(a.o.dtype);
-  const int64_t groups = (a.in + kA8Group - 1) / kA8Group;
-  const int64_t qsz = a.op == LIN_WGRAD ? a.rows * groups * kA8Group : ody_quant_bytes(a.kind, a.out * a.in);
+  if (a.o.c == a.a || a.o.c == a.q || a.o.c == a.scales) return fail(ODY_ERR_ARG, kOverlap);
+  const Spans s(a);
+  const int64_t asz = s.a.n * s.a.pitch, csz = s.c.n * s.c.pitch, qsz = s.q.bytes;
   a.o.alpha = alpha;
   Scope S;
   S.bufs.reserve(8);
@@ -127,7 +169,7 @@ int staged(LinearArgs a, float alpha) {
   void* const c = a.o.c;
   ODY_STAGE(S, a.a, (size_t)asz, true, &da);
   ODY_STAGE(S, a.q, (size_t)qsz, true, &dq);
-  if (a.scales) ODY_STAGE(S, a.scales, (size_t)(a.rows * groups), true, &ds);
+  if (a.scales) ODY_STAGE(S, a.scales, (size_t)s.scales.bytes, true, &ds);
   if (a.o.add && a.o.add != c) ODY_STAGE(S, a.o.add, (size_t)csz, true, &dadd);
   ODY_STAGE(S, c, (size_t)csz, a.o.add == c, &dc);
   if (a.o.add == c) dadd = dc;
@@ -151,14 +193,19 @@ int act8_args(int32_t fmt, const void* x, int32_t dt, int64_t rows, int64_t cols
   if (rows > kMaxDim || cols > kMaxDim) return fail(ODY_ERR_SHAPE, "linear: a dimension is too large");
   if (int rc = check_pitch(ld, cols, "the activation")) return rc;
   if (!x || !codes || !scales) return fail(ODY_ERR_ARG, "null pointer");
+  if (x == codes || x == scales || codes == scales) return fail(ODY_ERR_ARG, kOverlap);
   return ODY_OK;
 }
 
-int act8_device(const void* x, int32_t dt, const void* codes, const void* scales, const char* name) {
+int act8_device(const void* x, int32_t dt, int64_t rows, int64_t cols, int64_t ld, const void* codes, const void* scales,
+                const char* name) {
+  const int64_t es = dtype_size(dt), groups = ody_act8_groups(cols);
+  const Span sx = {x, rows, cols * es, ld * es}, sc = flat(codes, rows * groups * kA8Group), ss = flat(scales, rows * groups);
   if (!is_device_ptr(x) || !is_device_ptr(codes) || !is_device_ptr(scales))
     return fail(ODY_ERR_ARG, std::string(name) + " takes memory of the current GPU only");
   if (reinterpret_cast<uintptr_t>(codes) & 15u)
     return fail(ODY_ERR_ARG, std::string(name) + ": codes must be 16-byte aligned");
+  if (meet(sx, sc) || meet(sx, ss) || meet(sc, ss)) return fail(ODY_ERR_ARG, kOverlap);
   return aligned_to(x, dt, "the activation");
 }
 
@@ -170,7 +217,7 @@ extern "C" int ody_act8_save_on_stream(int32_t fmt, const void* x, int32_t dt, i
                                        uint8_t* codes, uint8_t* scales, void* stream) {
   return guarded([&]() -> int {
     if (int rc = act8_args(fmt, x, dt, rows, cols, ldx, codes, scales)) return rc;
-    if (int rc = act8_device(x, dt, codes, scales, "ody_act8_save_on_stream")) return rc;
+    if (int rc = act8_device(x, dt, rows, cols, ldx, codes, scales, "ody_act8_save_on_stream")) return rc;
     return launched(launch_act8_save(fmt, x, dt, rows, cols, ldx, codes, scales, (cudaStream_t)stream), "launch_act8_save");
   });
 }
@@ -179,7 +226,7 @@ extern "C" int ody_act8_load_on_stream(int32_t fmt, const uint8_t* codes, const 
                                        int64_t cols, void* out, int32_t dt, int64_t ldo, void* stream) {
   return guarded([&]() -> int {
     if (int rc = act8_args(fmt, out, dt, rows, cols, ldo, codes, scales)) return rc;
-    if (int rc = act8_device(out, dt, codes, scales, "ody_act8_load_on_stream")) return rc;
+    if (int rc = act8_device(out, dt, rows, cols, ldo, codes, scales, "ody_act8_load_on_stream")) return rc;
     return launched(launch_act8_load(fmt, codes, scales, rows, cols, out, dt, ldo, (cudaStream_t)stream), "launch_act8_load");
   });
 }
@@ -195,7 +242,7 @@ extern "C" int ody_act8_save(int32_t fmt, const void* x, int32_t dt, int64_t row
     ODY_STAGE(S, x, (size_t)(rows * cols) * dtype_size(dt), true, &dx);
     ODY_STAGE(S, codes, (size_t)(rows * groups * kA8Group), false, &dc);
     ODY_STAGE(S, scales, (size_t)(rows * groups), false, &ds);
-    if (int rc = act8_device(dx, dt, dc, ds, "ody_act8_save")) return rc;
+    if (int rc = act8_device(dx, dt, rows, cols, cols, dc, ds, "ody_act8_save")) return rc;
     if (int rc = launched(launch_act8_save(fmt, dx, dt, rows, cols, cols, (uint8_t*)dc, (uint8_t*)ds, S.st), "launch_act8_save"))
       return rc;
     ODY_CUDA(S.copy_out(codes));
@@ -216,7 +263,7 @@ extern "C" int ody_act8_load(int32_t fmt, const uint8_t* codes, const uint8_t* s
     ODY_STAGE(S, codes, (size_t)(rows * groups * kA8Group), true, &dc);
     ODY_STAGE(S, scales, (size_t)(rows * groups), true, &ds);
     ODY_STAGE(S, out, (size_t)(rows * cols) * dtype_size(dt), false, &dx);
-    if (int rc = act8_device(dx, dt, dc, ds, "ody_act8_load")) return rc;
+    if (int rc = act8_device(dx, dt, rows, cols, cols, dc, ds, "ody_act8_load")) return rc;
     if (int rc = launched(launch_act8_load(fmt, (const uint8_t*)dc, (const uint8_t*)ds, rows, cols, dx, dt, cols, S.st),
                           "launch_act8_load"))
       return rc;

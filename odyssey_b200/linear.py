@@ -14,7 +14,9 @@ where they lie.  Activations and gradients are float32, float16 or bfloat16
 arrays whose last axis is the feature axis; leading axes are tokens.  CUDA
 tensors run on torch's current stream of their device without waiting, host
 arrays (numpy, or torch on the CPU; bfloat16 numpy data as uint16 with
-dtype='bfloat16') are staged and the call returns when done.
+dtype='bfloat16') are staged and the call returns when done.  A result may not
+share memory with an operand (linear_wgrad8's add=out apart); such a call is
+refused.
 """
 import ctypes as C
 from dataclasses import dataclass

@@ -48,3 +48,56 @@ def test_host_results_over_their_operands(ody):
     L.check(lib.ody_adamw_step(*args, 1000, 1, 1e-3, 0.9, 0.999, 1e-8, 0.01, args[0], args[2], args[3]))
     for got, w in zip((p, m, v), want):
         assert np.array_equal(got, w)
+
+
+def test_device_results_that_overlap_operands_are_refused(ody):
+    """A result that shares a byte with an operand is turned away; columns of
+    one buffer that lie between the operand's are not."""
+    from odyssey_b200 import _lib as L
+    lib = L.lib()
+    st = torch.cuda.current_stream().cuda_stream
+    rng = np.random.default_rng(3)
+    out, inn, rows, ld = 32, 64, 6, 200
+    q = torch.from_numpy(R.random_weight(rng, R.NVFP4, out, inn)).cuda()
+    w = ody.QuantizedTensor(q, R.NVFP4, out * inn)
+    buf = torch.randn(3 * rows, ld, device="cuda")
+    before = buf.clone()
+
+    def call(y, ldy, x=(0, 0), ldx=ld, n=rows, q=q.data_ptr(), ts=None):
+        at = lambda p: buf.data_ptr() + 4 * (p[0] * ld + p[1])
+        return lib.ody_fp4_linear_on_stream(R.NVFP4, q, ts, 1.0, out, inn, at(x), L.F32, n, ldx, at(y), L.F32, ldy, None, 0, st)
+
+    for y, ldy in (((0, 0), ld), ((0, 63), ld), ((0, ld - 31), ld), ((rows - 1, 63), ld), ((rows - 1, 10), 2 * ld),
+                   ((0, 64), ld - 1), ((0, 100), 130), ((0, 150), 2 * ld + 49)):
+        x = (1, 0) if y == (0, ld - 31) else (0, 0)  # there y's rows end in the first column of x's next ones
+        assert call(y, ldy, x) == L.ERR_ARG, (y, ldy)
+    whole = ody.QuantizedTensor(buf.view(torch.uint8).view(-1)[:q.numel()], R.NVFP4, out * inn)
+    assert call((0, 60), ld, (rows, 0), q=whole.data.data_ptr()) == L.ERR_ARG
+    assert call((0, 0), ld, (rows, 0), ts=buf.data_ptr() + 4 * ld) == L.ERR_ARG
+    torch.cuda.synchronize()
+    assert torch.equal(buf, before)
+    for y, ldy, x in (((0, 64), ld, (0, 0)), ((0, ld - 32), ld, (1, 0)), ((0, 64), 2 * ld, (1, 0)), ((rows, 0), ld, (0, 0)), ((rows, 0), 32, (0, 0))):
+        want = ody.fp4_linear(buf[x[0]:x[0] + rows, :inn].clone(), w)
+        assert call(y, ldy, x) == L.OK
+        got = torch.as_strided(buf, (rows, out), (ldy, 1), y[0] * ld + y[1])
+        assert torch.equal(got, want)
+        buf.copy_(before)
+    # through Python: a view of the input's memory, and of the activation's
+    x = torch.randn(8, 64, device="cuda")
+    for o in (x.view(-1)[:8 * 32].view(8, 32), x.view(-1)[64:64 + 8 * 32].view(8, 32), x.view(-1)[256:].view(8, 32)):
+        with pytest.raises(ody.OdysseyError, match="overlap an operand"):
+            ody.fp4_linear(x, w, out=o)
+    big = torch.zeros(4096, dtype=torch.uint8, device="cuda")
+    a = ody.Activation8(big[:512].view(8, 64), torch.full((8, 2), 127, dtype=torch.uint8, device="cuda"), 8, 64)
+    for at in (0, 256, 508):
+        with pytest.raises(ody.OdysseyError, match="overlap an operand"):
+            ody.load_activation8(a, "float32", out=big[at:at + 2048].view(torch.float32).view(8, 64))
+    ody.load_activation8(a, "float32", out=big[512:2560].view(torch.float32).view(8, 64))
+    with pytest.raises(ody.OdysseyError, match="overlap an operand"):
+        ody.linear_wgrad8(x[:, :4].contiguous(), a, out=big[508:1020].view(torch.bfloat16).view(4, 64), out_dtype="bfloat16")
+    dy = torch.randn(8, 32, device="cuda")
+    acc = torch.randn(33, 64, device="cuda")
+    with pytest.raises(ody.OdysseyError, match="overlap an operand"):
+        ody.linear_wgrad8(dy, a, add=acc[:32], out=acc[1:])
+    want = ody.linear_wgrad8(dy, a, add=acc[:32].clone())
+    assert torch.equal(ody.linear_wgrad8(dy, a, add=acc[:32], out=acc[:32]), want)

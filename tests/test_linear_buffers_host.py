@@ -65,3 +65,31 @@ def test_load_refuses_a_shape_of_other_elements(ody):
         a = ody.Activation8(codes, scales, 3, 40, shape=shape)
         refused(ody, L.ERR_SHAPE, "120 elements", ody.load_activation8, a)
         refused(ody, L.ERR_SHAPE, "120 elements", ody.load_activation8, a, out=np.empty(shape, np.float32), dtype="float32")
+
+
+def test_results_that_are_operands_are_refused(ody):
+    """By name of the caller's buffers, before anything is copied or launched."""
+    from odyssey_b200 import _lib as L
+    import torch
+    n = 32
+    w = ody.QuantizedTensor(np.zeros(L.quant_bytes(L.Q_NVFP4, n * n), np.uint8), L.Q_NVFP4, n * n)
+    x = np.ones((n, n), np.float32)
+    for fn in (ody.fp4_linear, ody.fp4_linear_dgrad):
+        refused(ody, L.ERR_ARG, "must not be or overlap an operand", fn, x, w, out=x)
+        t = torch.ones(n, n)
+        refused(ody, L.ERR_ARG, "must not be or overlap an operand", fn, t, ody.QuantizedTensor(torch.from_numpy(w.data), w.kind, n * n),
+                out=t)
+    a = ody.Activation8(np.zeros((n, n), np.uint8), np.zeros((n, 1), np.uint8), n, n)
+    refused(ody, L.ERR_ARG, "must not be or overlap an operand", ody.linear_wgrad8, x, a, out=x)
+    lib, p = L.lib(), x.ctypes.data
+    c, s = a.codes.ctypes.data, a.scales.ctypes.data
+    assert lib.ody_fp4_linear(L.Q_NVFP4, p, 1.0, n, n, x.ctypes.data + 64, L.F32, 1, p, L.F32) == L.ERR_ARG
+    assert lib.ody_linear_wgrad8(0, c, s, 1, n, p, L.F32, 1, 1.0, None, c, L.F32) == L.ERR_ARG
+    assert lib.ody_linear_wgrad8(0, c, s, 1, n, p, L.F32, 1, 1.0, None, s, L.F32) == L.ERR_ARG
+    for act8 in (lambda x, c, s: lib.ody_act8_save(0, x, L.F32, 1, n, c, s), lambda x, c, s: lib.ody_act8_load(0, c, s, 1, n, x, L.F32)):
+        assert act8(p, p, s) == L.ERR_ARG and act8(p, c, p) == L.ERR_ARG and act8(p, c, c) == L.ERR_ARG
+    # neither accumulation in place nor neighbouring buffers are (without a GPU they fail behind the checks)
+    if not torch.cuda.is_available():
+        acc = np.zeros((n, n), np.float32)
+        refused(ody, L.ERR_CUDA, None, ody.linear_wgrad8, x[:, :16], a, add=acc[:16], out=acc[:16])
+        refused(ody, L.ERR_CUDA, None, ody.fp4_linear, x[:16], w, out=x[16:])
