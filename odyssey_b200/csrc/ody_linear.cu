@@ -213,12 +213,14 @@ __global__ void __launch_bounds__(256) medium_kernel(const LinearArgs p) {
 }
 
 static int lin_sms() {
-  static int n[64] = {0};
-  int dev = 0;
+  static std::atomic<int> known[kMaxDevices];
+  int dev = 0, n = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return 148;
-  if (!n[dev]) cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev);
-  return n[dev] ? n[dev] : 148;
+  if (dev < 0 || dev >= kMaxDevices) return 148;
+  if ((n = known[dev].load(std::memory_order_relaxed))) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 struct MediumPlan {
@@ -243,14 +245,8 @@ template <int OP, int KIND, int DT>
 static cudaError_t launch_medium(const LinearArgs& a, const MediumPlan& p, cudaStream_t st) {
   constexpr int smem = 2 * (bf16_parts(DT) + 1) * kMTile;
   static_assert(smem >= kMT * kMSumPitch * 4, "the sums fit");
-  static bool set[64] = {false};  // per device; setting it twice is harmless
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(medium_kernel<OP, KIND, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) set[dev] = true;
-  }
+  static PerDevice set;
+  if (const cudaError_t e = allow_shared(set, (const void*)medium_kernel<OP, KIND, DT>, smem)) return e;
   if (p.ranks == 1) {
     medium_kernel<OP, KIND, DT><<<(unsigned)p.tiles, 256, smem, st>>>(a);
     return cudaGetLastError();

@@ -5,7 +5,24 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace ody {
+
+// Lets a kernel take `bytes` of dynamic shared memory on the current device;
+// `set` is the kernel's own.  `bytes` is the most that any launch of it takes:
+// with one number per kernel two threads may set it in any order.
+constexpr int kMaxDevices = 64;
+using PerDevice = std::atomic<bool>[kMaxDevices];
+inline cudaError_t allow_shared(PerDevice& set, const void* kernel, int bytes) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool known = dev >= 0 && dev < kMaxDevices;
+  if (known && set[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && known) set[dev].store(true, std::memory_order_release);
+  return e;
+}
 
 // C[m, n] = alpha * *tscale * sum_r A(m, r) B(n, r) (+ add[m, n]), rounded
 // once to the output's type.

@@ -6,6 +6,7 @@
 #include "ody_host.h"
 #include "ody_linear.h"
 #include "ody_linear_gemm.h"
+#include "ody_linear_rows.h"
 
 using namespace ody;
 
@@ -354,5 +355,12 @@ extern "C" int ody_linear_status(void* stream) {
 // out after so many cycles.
 extern "C" int odyx_linear_wait_selftest(int64_t cycles, void* stream) {
   ODY_CUDA(launch_wait_selftest(cycles, (cudaStream_t)stream));
+  return ODY_OK;
+}
+
+// Test hook (not part of include/odyssey_mp.h): what a few-row kernel may take
+// of shared memory, as the calls so far have set it.
+extern "C" int odyx_linear_rows_limit(int32_t* bytes) {
+  ODY_CUDA(rows_shared_limit(bytes));
   return ODY_OK;
 }

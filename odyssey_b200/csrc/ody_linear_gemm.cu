@@ -796,15 +796,8 @@ cudaError_t prepare_w4(PrepareArgs& p, int dtype, int x_ctas, int sms, cudaStrea
 
 template <bool AMN, bool BMN, int DT>
 cudaError_t run_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& g, int sms, cudaStream_t st) {
-  static bool set[64] = {false};  // per device; setting it twice is harmless
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !set[dev]) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(gemm_kernel<AMN, BMN, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) set[dev] = true;
-  }
+  static PerDevice set;
+  if (const cudaError_t e = allow_shared(set, (const void*)gemm_kernel<AMN, BMN, DT>, kGemmSmem)) return e;
   // with whole tiles only, no more pairs than tiles
   const int64_t shares = ((int64_t)g.shared * g.total + g.deal - 1) / g.deal;
   const int64_t work = g.tiles_m * (int64_t)g.tiles_n > g.shared ? sms / 2 : shares;

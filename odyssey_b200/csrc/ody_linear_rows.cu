@@ -569,16 +569,11 @@ int cluster_for(int64_t tiles, int64_t steps, int ctas) {
   return cluster;
 }
 
+// smem: this launch's shared memory, most: the most of any launch of the kernel
 template <void (*kernel)(const RowArgs)>
-cudaError_t launch_rows(const RowArgs& a, int64_t tiles, int cluster, int smem, cudaStream_t st) {
-  static int most[64] = {0};  // of this kernel, per device; setting it twice is harmless
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || most[dev] < smem) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) most[dev] = smem;
-  }
+cudaError_t launch_rows(const RowArgs& a, int64_t tiles, int cluster, int smem, int most, cudaStream_t st) {
+  static PerDevice set;
+  if (const cudaError_t e = allow_shared(set, (const void*)kernel, most)) return e;
   if (cluster == 1) {
     kernel<<<(unsigned)tiles, kRowThreads, smem, st>>>(a);
     return cudaGetLastError();
@@ -604,16 +599,16 @@ cudaError_t launch_one(const LinearArgs& l, RowArgs a, int sms, cudaStream_t st)
     const int64_t runs = std::min<int64_t>(units, 2 * sms / cluster);
     while (1 << a.cluster < cluster) a.cluster++;
     a.per = (int)(units / runs), a.extra = (int)(units % runs);
-    return launch_rows<rows_forward_kernel<KIND, DT, NT>>(
-        a, runs, cluster,
-        kTableBytes<S::TABLES> + kRowWarps * (S::DEPTH * Ring<KIND, 256, kTileR>::BYTES + S::SUMS * 4), st);
+    constexpr int smem = kTableBytes<S::TABLES> + kRowWarps * (S::DEPTH * Ring<KIND, 256, kTileR>::BYTES + S::SUMS * 4);
+    return launch_rows<rows_forward_kernel<KIND, DT, NT>>(a, runs, cluster, smem, smem, st);
   }
   if constexpr (NT <= 2) {
     constexpr int ring = kTableBytes<true> + kRowWarps * kDepth * Ring<KIND, kDK, kTileR>::BYTES, sums = kRowWarps * NT * 8 * kRedPitch * 4;
     const int64_t tiles = (a.in + kDK - 1) / kDK, steps = (a.out + kTileR - 1) / kTileR;
     const int cluster = cluster_for(tiles, (steps + kRowWarps - 1) / kRowWarps, 2 * sms);
     a.keep = steps > 32 * (int64_t)kRowWarps * cluster;
-    return launch_rows<rows_dgrad_kernel<KIND, DT, NT>>(a, tiles, cluster, a.keep ? ring + sums : std::max(ring, sums), st);
+    return launch_rows<rows_dgrad_kernel<KIND, DT, NT>>(a, tiles, cluster, a.keep ? ring + sums : std::max(ring, sums),
+                                                        ring + sums, st);
   }
   return cudaErrorInvalidValue;
 }
@@ -634,6 +629,13 @@ cudaError_t launch_dt(const LinearArgs& l, const RowArgs& a, int sms, cudaStream
 }
 
 }  // namespace
+
+cudaError_t rows_shared_limit(int* bytes) {
+  cudaFuncAttributes f;
+  const cudaError_t e = cudaFuncGetAttributes(&f, rows_dgrad_kernel<Q_MXFP4, DT_BF16, 1>);
+  *bytes = e == cudaSuccess ? f.maxDynamicSharedSizeBytes : 0;
+  return e;
+}
 
 bool few_rows(const LinearArgs& a) {
   if (a.op == LIN_WGRAD) return false;

@@ -5,5 +5,7 @@
 
 namespace ody {
 bool few_rows(const LinearArgs& a);
+// shared memory that one row's backward kernel (MXFP4, bfloat16) may take on the current device
+cudaError_t rows_shared_limit(int* bytes);
 cudaError_t launch_few_rows(const LinearArgs& a, int sms, cudaStream_t st);
 }  // namespace ody

@@ -101,3 +101,71 @@ def test_device_results_that_overlap_operands_are_refused(ody):
         ody.linear_wgrad8(dy, a, add=acc[:32], out=acc[1:])
     want = ody.linear_wgrad8(dy, a, add=acc[:32].clone())
     assert torch.equal(ody.linear_wgrad8(dy, a, add=acc[:32], out=acc[:32]), want)
+
+
+def run_python(code):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("done"), r.stdout + r.stderr
+
+
+LAYERS = """
+import ctypes as C, threading, torch, odyssey_b200 as ody
+def layer(kind, block, size, out, inn, rows, dtype):
+    g = torch.Generator(device="cuda").manual_seed(out)
+    q = torch.randint(0, 120, (out * inn // block * size,), dtype=torch.uint8, device="cuda", generator=g)
+    return ody.QuantizedTensor(q, kind, out * inn), torch.randn(rows, out, device="cuda", generator=g).to(dtype)
+"""
+
+
+def test_shared_memory_limit_is_one_number(ody):
+    """A few-row backward product over a long reduction takes more shared
+    memory than one over a short one.  What a kernel may take does not depend
+    on which came first, so threads that set it cross without harm."""
+    run_python(LAYERS + """
+def limit():
+    n = C.c_int32(0)
+    assert ody.lib().odyx_linear_rows_limit(C.byref(n)) == 0
+    return n.value
+w, dy = layer(6, 32, 17, 64, 64, 1, torch.bfloat16)
+ody.fp4_linear_dgrad(dy, w)
+short = limit()
+w, dy = layer(6, 32, 17, 70000, 64, 1, torch.bfloat16)
+ody.fp4_linear_dgrad(dy, w)
+torch.cuda.synchronize()
+assert short == limit(), (short, limit())
+print("done")
+""")
+
+
+def test_first_calls_from_threads_at_once(ody):
+    """A process's first calls of every kind and type, short and long
+    reductions at once from two threads each (four in all), give what later calls give."""
+    run_python(LAYERS + """
+errors, results = [], []
+for kind, block, size in ((6, 32, 17), (7, 16, 9), (9, 32, 17)):
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        for rows in (1, 4, 300):
+            sets = [layer(kind, block, size, out, inn, rows, dtype) for out, inn in ((64, 64), (20000, 64))] * 2
+            torch.cuda.synchronize()
+            start, got = threading.Barrier(len(sets)), [None] * len(sets)
+            def call(i):
+                try:
+                    start.wait()
+                    with torch.cuda.stream(torch.cuda.Stream()):
+                        got[i] = (ody.fp4_linear_dgrad(sets[i][1], sets[i][0]),)
+                        torch.cuda.current_stream().synchronize()
+                except Exception as e:
+                    errors.append(repr(e))
+            ts = [threading.Thread(target=call, args=(i,)) for i in range(len(sets))]
+            [t.start() for t in ts]
+            [t.join() for t in ts]
+            assert not errors, errors
+            for (w, dy), (y,) in zip(sets, got):
+                assert torch.equal(ody.fp4_linear_dgrad(dy, w), y)
+torch.cuda.synchronize()
+print("done")
+""")
