@@ -416,7 +416,7 @@ int ody_dequant_bf16(const void* q, int64_t n, float* out);   /* the exact BF16 
  * allocation, no synchronisation): the caller keeps the buffers until the
  * work is done, and gives every call that may overlap another one a
  * workspace of its own, 256-byte aligned, of at least
- * ody_linear_workspace(op, ...) bytes (may be 0).  tensor_scale (a device
+ * ody_linear_workspace_of(op, kind, ...) bytes (may be 0).  tensor_scale (a device
  * float, or NULL for 1) is ODY_Q_NVFP4_TENSOR's; results are multiplied by
  * alpha * *tensor_scale.  Outputs must not overlap inputs, except that add
  * may be dw itself (accumulation in place); columns of one wide buffer do not
@@ -425,8 +425,13 @@ int ody_dequant_bf16(const void* q, int64_t n, float* out);   /* the exact BF16 
 #define ODY_LINEAR_FORWARD 0
 #define ODY_LINEAR_DGRAD 1
 #define ODY_LINEAR_WGRAD 2
-/* workspace bytes of one call (-1: bad arguments); act_dtype is x's or dy's */
+/* Workspace bytes of one call (-1: bad arguments); act_dtype is x's or dy's.
+ * The first form is enough for a weight of any kind, the second is what a
+ * call with this kind takes (few rows of NVFP4 with a width of 16s take none
+ * where the other kinds may). */
 int64_t ody_linear_workspace(int32_t op, int64_t rows, int64_t out_features, int64_t in_features, int32_t act_dtype);
+int64_t ody_linear_workspace_of(int32_t op, int32_t kind, int64_t rows, int64_t out_features, int64_t in_features,
+                                int32_t act_dtype);
 /* Waits for `stream` and reports what the calls on the current GPU cannot
  * return: ODY_ERR_DEVICE_BOUNDS if a wait inside one of their kernels ran out
  * (each is bounded by 2 s; results of that call are then incomplete) since

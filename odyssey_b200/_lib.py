@@ -128,6 +128,7 @@ _SIGS = {
     "ody_quantize": (C.c_int, [_i32, _p, _i32, _i64, _p, _p]),
     "ody_dequantize": (C.c_int, [_i32, _p, _i64, C.c_float, _p]),
     "ody_linear_workspace": (_i64, [_i32, _i64, _i64, _i64, _i32]),
+    "ody_linear_workspace_of": (_i64, [_i32, _i32, _i64, _i64, _i64, _i32]),
     "ody_linear_status": (C.c_int, [_p]),
     "ody_fp4_linear_on_stream": (C.c_int, [_i32, _p, _p, C.c_float, _i64, _i64, _p, _i32, _i64, _i64, _p, _i32, _i64,
                                            _p, C.c_size_t, _p]),

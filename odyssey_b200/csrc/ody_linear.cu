@@ -293,10 +293,7 @@ static cudaError_t launch_medium_w4(const LinearArgs& a, const MediumPlan& p, cu
 constexpr int64_t kMediumRounds = 12;
 static bool medium_product(const LinearArgs& a) { return medium_plan(a, lin_sms()).rounds <= kMediumRounds; }
 
-// (of any kind: the query does not name one, so widths are taken to be in 32s)
-int64_t linear_workspace(const LinearArgs& a) {
-  return medium_product(a) || (few_rows(a) && a.in % 32 == 0) ? 0 : gemm_workspace(a, lin_sms());
-}
+int64_t linear_workspace(const LinearArgs& a) { return few_rows(a) || medium_product(a) ? 0 : gemm_workspace(a, lin_sms()); }
 
 cudaError_t launch_linear(const LinearArgs& a, void* ws, cudaStream_t st) {
   const int sms = lin_sms();

@@ -53,7 +53,7 @@ struct LinearArgs {
 enum : int { A8_E4M3 = 0, A8_E5M2 = 1 };
 constexpr int kA8Group = 32;
 
-// bytes of workspace launch_linear may use for these shapes and types,
+// bytes of workspace launch_linear uses for these shapes, types and kind,
 // whatever the pointers' alignment and the strides
 int64_t linear_workspace(const LinearArgs& a);
 cudaError_t launch_linear(const LinearArgs& a, void* ws, cudaStream_t st);

@@ -274,15 +274,22 @@ extern "C" int ody_act8_load(int32_t fmt, const uint8_t* codes, const uint8_t* s
   });
 }
 
-extern "C" int64_t ody_linear_workspace(int32_t op, int64_t rows, int64_t out, int64_t in, int32_t act_dtype) {
+extern "C" int64_t ody_linear_workspace_of(int32_t op, int32_t kind, int64_t rows, int64_t out, int64_t in,
+                                           int32_t act_dtype) {
   LinearArgs a{};
-  if (op < LIN_FORWARD || op > LIN_WGRAD || rows <= 0 || out <= 0 || in <= 0 || rows > kMaxDim || out > kMaxDim ||
+  if (op < LIN_FORWARD || op > LIN_WGRAD || (op != LIN_WGRAD && !is_w4(kind)) || rows <= 0 || out <= 0 || in <= 0 || rows > kMaxDim || out > kMaxDim ||
       in > kMaxDim || act_dtype < DT_F32 || act_dtype > DT_BF16)
     return -1;
   a.op = op;
   a.rows = rows, a.out = out, a.in = in;
   a.a_dtype = act_dtype;
+  a.kind = kind;
   return linear_workspace(a);
+}
+
+// the kind that fewest widths are whole blocks of asks for the most
+extern "C" int64_t ody_linear_workspace(int32_t op, int64_t rows, int64_t out, int64_t in, int32_t act_dtype) {
+  return ody_linear_workspace_of(op, ODY_Q_MXFP4, rows, out, in, act_dtype);
 }
 
 #define ODY_W4_PAIR(NAME, OP, ACT, OUT, ACOLS, CCOLS)                                                               \

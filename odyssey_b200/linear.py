@@ -166,8 +166,8 @@ def _enqueue(index, fn, *args):
 
 
 @lru_cache(maxsize=4096)
-def _workspace_bytes(device_index, op, rows, out, inn, code):
-    return int(L.lib().ody_linear_workspace(op, rows, out, inn, code))
+def _workspace_bytes(device_index, op, kind, rows, out, inn, code):
+    return int(L.lib().ody_linear_workspace_of(op, kind, rows, out, inn, code))
 
 
 def _workspace(a, n):
@@ -219,7 +219,7 @@ def _product(name, op, x, w, out, out_dtype, dtype, what):
         else:
             alpha = w.tensor_scale
     index = r.a.get_device()
-    ws, at, n = _workspace(r.a, _workspace_bytes(index, op, r.rows, nout, nin, r.code))
+    ws, at, n = _workspace(r.a, _workspace_bytes(index, op, w.kind, r.rows, nout, nin, r.code))
     _enqueue(index, lib.ody_fp4_linear_on_stream if op == L.LINEAR_FORWARD else lib.ody_fp4_linear_dgrad_on_stream, w.kind,
              data.data_ptr(), ts, alpha, nout, nin, r.ptr, r.code, r.rows, r.ld, y.data_ptr(), code, other, at, n)
     return y
@@ -304,7 +304,7 @@ def linear_wgrad8(dy, a, add=None, alpha=1.0, out=None, out_dtype=None, dtype=No
     fmt, lib = FORMATS8[a.format], L.lib()
     if r.cuda:
         index = r.a.get_device()
-        ws, at, n = _workspace(r.a, _workspace_bytes(index, L.LINEAR_WGRAD, r.rows, r.cols, a.cols, r.code))
+        ws, at, n = _workspace(r.a, _workspace_bytes(index, L.LINEAR_WGRAD, fmt, r.rows, r.cols, a.cols, r.code))
         _enqueue(index, lib.ody_linear_wgrad8_on_stream, fmt, codes.data_ptr(), scales.data_ptr(), a.rows, a.cols, r.ptr,
                  r.code, r.cols, r.ld, alpha, None if add is None else add.data_ptr(), y.data_ptr(), code, at, n)
     else:

@@ -169,3 +169,30 @@ for kind, block, size in ((6, 32, 17), (7, 16, 9), (9, 32, 17)):
 torch.cuda.synchronize()
 print("done")
 """)
+
+
+def test_few_rows_take_no_workspace(ody):
+    """NVFP4 with a width of 16s that is not one of 32s: the call brings none
+    and allocates nothing but its result."""
+    from odyssey_b200 import _lib as L
+    rng = np.random.default_rng(4)
+    out, inn = 4096, 4080
+    q = R.random_weight(rng, R.NVFP4, out, inn)
+    w = ody.QuantizedTensor(torch.from_numpy(q).cuda(), R.NVFP4, out * inn)
+    w64 = R.weight(R.NVFP4, q, out, inn)
+    for rows, op, fn, cols, others, m in ((8, L.LINEAR_FORWARD, ody.fp4_linear, inn, out, w64.T),
+                                          (4, L.LINEAR_DGRAD, ody.fp4_linear_dgrad, out, inn, w64)):
+        x = torch.from_numpy(rng.standard_normal((rows, cols)).astype(np.float32)).cuda()
+        x64 = R.to64(x)
+        fn(x, w)  # loads the kernels
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        y = fn(x, w)
+        assert torch.cuda.max_memory_allocated() - before < 2 * 4 * rows * others
+        R.check(y, x64 @ m, R.tolerance(np.abs(x64) @ np.abs(m), cols, x64 @ m, "float32"))
+        z = torch.empty_like(y)
+        entry = L.lib().ody_fp4_linear_on_stream if op == L.LINEAR_FORWARD else L.lib().ody_fp4_linear_dgrad_on_stream
+        assert entry(w.kind, w.data.data_ptr(), None, 1.0, out, inn, x.data_ptr(), L.F32, rows, cols, z.data_ptr(), L.F32,
+                     others, None, 0, torch.cuda.current_stream().cuda_stream) == L.OK
+        assert torch.equal(z, y)

@@ -93,3 +93,24 @@ def test_results_that_are_operands_are_refused(ody):
         acc = np.zeros((n, n), np.float32)
         refused(ody, L.ERR_CUDA, None, ody.linear_wgrad8, x[:, :16], a, add=acc[:16], out=acc[:16])
         refused(ody, L.ERR_CUDA, None, ody.fp4_linear, x[:16], w, out=x[16:])
+
+
+def test_workspace_of_a_kind(ody):
+    """Few rows of whole blocks take none, whatever the other kinds' blocks
+    are; the query without a kind covers every kind."""
+    from odyssey_b200 import _lib as L
+    of, any_kind = L.lib().ody_linear_workspace_of, L.lib().ody_linear_workspace
+    kinds = (L.Q_MXFP4, L.Q_NVFP4, L.Q_NVFP4_TENSOR, L.Q_MXFP4_OCP)
+    for op, most in ((L.LINEAR_FORWARD, 32), (L.LINEAR_DGRAD, 16)):
+        for dtype, parts in ((L.F32, 3), (L.F16, 2), (L.BF16, 1)):
+            for rows in (1, most // parts, most // parts + 1, 200, 2048):
+                for inn in (8192, 8176, 8168):
+                    need = {k: of(op, k, rows, 8192, inn, dtype) for k in kinds}
+                    assert any_kind(op, rows, 8192, inn, dtype) == max(need.values())
+                    for k in kinds:
+                        block = 32 if k in (L.Q_MXFP4, L.Q_MXFP4_OCP) else 16
+                        few = rows * parts <= most and inn % block == 0
+                        assert (need[k] == 0) == few, (op, dtype, rows, inn, k)
+    for bad in ((3, 6, 1, 1, 1, 0), (0, 3, 1, 1, 1, 0), (1, 10, 1, 1, 1, 0), (0, 6, 0, 1, 1, 0), (0, 6, 1, 1, 1, 7)):
+        assert of(*bad) == -1
+    assert of(L.LINEAR_WGRAD, L.A8_E5M2, 8192, 4096, 4096, L.BF16) == any_kind(L.LINEAR_WGRAD, 8192, 4096, 4096, L.BF16) > 0
