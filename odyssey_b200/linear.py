@@ -51,6 +51,11 @@ def _code(dtype):
     return c
 
 
+def _check_bytes(b, what):
+    if (b if L.is_torch(b) else np.asarray(b)).dtype.itemsize != 1:
+        raise L.OdysseyError(f"{what} must be uint8", L.ERR_DTYPE)
+
+
 @dataclass
 class Activation8:
     """An activation in 8 bits: codes [rows, 32 * groups] and one scale byte
@@ -74,8 +79,7 @@ class Activation8:
             if L.numel(b) != n:
                 raise L.OdysseyError("codes and scales do not have the bytes of the activation's rows and columns",
                                      L.ERR_SHAPE)
-            if (b.dtype.itemsize if L.is_torch(b) else np.asarray(b).itemsize) != 1:
-                raise L.OdysseyError("codes and scales must be uint8", L.ERR_DTYPE)
+            _check_bytes(b, "codes and scales")
 
 
 class _Rows:
@@ -199,6 +203,7 @@ def _product(name, op, x, w, out, out_dtype, dtype, what):
     data = w.data
     if L.numel(data) != need:
         raise L.OdysseyError(f"quantised buffer has {L.numel(data)} bytes, expected {need}", L.ERR_SHAPE)
+    _check_bytes(data, "the weight's buffer")
     code = r.code if out_dtype is None else _code(out_dtype)
     y = _out(r, out, (*r.lead, other), code, "out")
     lib = L.lib()

@@ -114,3 +114,18 @@ def test_workspace_of_a_kind(ody):
     for bad in ((3, 6, 1, 1, 1, 0), (0, 3, 1, 1, 1, 0), (1, 10, 1, 1, 1, 0), (0, 6, 0, 1, 1, 0), (0, 6, 1, 1, 1, 7)):
         assert of(*bad) == -1
     assert of(L.LINEAR_WGRAD, L.A8_E5M2, 8192, 4096, 4096, L.BF16) == any_kind(L.LINEAR_WGRAD, 8192, 4096, 4096, L.BF16) > 0
+
+
+def test_weights_that_are_not_bytes_are_refused(ody):
+    """As many elements as the weight has bytes, of another size, are not its
+    bytes."""
+    from odyssey_b200 import _lib as L
+    import torch
+    n = L.quant_bytes(L.Q_NVFP4, 8 * 16)
+    x = np.ones((2, 16), np.float32)
+    for dtype in (np.int16, np.float32, np.int64):
+        w = ody.QuantizedTensor(np.zeros(n, dtype), L.Q_NVFP4, 8 * 16)
+        refused(ody, L.ERR_DTYPE, "must be uint8", ody.fp4_linear, x, w)
+        refused(ody, L.ERR_DTYPE, "must be uint8", ody.fp4_linear_dgrad, x[:, :8], w)
+        t = ody.QuantizedTensor(torch.from_numpy(w.data), L.Q_NVFP4, 8 * 16)
+        refused(ody, L.ERR_DTYPE, "must be uint8", ody.fp4_linear, torch.from_numpy(x), t)
