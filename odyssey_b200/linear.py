@@ -16,7 +16,8 @@ tensors run on torch's current stream of their device without waiting, host
 arrays (numpy, or torch on the CPU; bfloat16 numpy data as uint16 with
 dtype='bfloat16') are staged and the call returns when done.  A result may not
 share memory with an operand (linear_wgrad8's add=out apart); such a call is
-refused.
+refused.  The gradients are calls of their own: no autograd graph is recorded,
+and a product of a tensor that requires one is refused while gradients are on.
 """
 import ctypes as C
 from dataclasses import dataclass
@@ -54,6 +55,14 @@ def _code(dtype):
 def _check_bytes(b, what):
     if (b if L.is_torch(b) else np.asarray(b)).dtype.itemsize != 1:
         raise L.OdysseyError(f"{what} must be uint8", L.ERR_DTYPE)
+
+
+def _no_graph(name, *buffers):
+    """Refuses tensors whose gradient would be lost: nothing here records one."""
+    for b in buffers:
+        if getattr(b, "requires_grad", False) and L._torch().is_grad_enabled():
+            raise L.OdysseyError(f"{name} records no gradient: detach its tensors or call it under torch.no_grad() "
+                                 "(the layer's gradients are fp4_linear_dgrad and linear_wgrad8)", L.ERR_ARG)
 
 
 @dataclass
@@ -198,6 +207,7 @@ def _weight(name, op, kind, numel, features):
 def _product(name, op, x, w, out, out_dtype, dtype, what):
     if not isinstance(w, QuantizedTensor) or w.kind not in _BLOCK:
         raise L.OdysseyError(f"{name} takes a weight of the 4-bit kinds", L.ERR_ARG)
+    _no_graph(name, x, out, w.tensor_scale)
     r = _Rows(x, dtype, what)
     other, nout, nin, need = _weight(name, op, w.kind, w.original_numel, r.cols)
     data = w.data
@@ -291,6 +301,7 @@ def linear_wgrad8(dy, a, add=None, alpha=1.0, out=None, out_dtype=None, dtype=No
     result's type; it may be `out` (accumulation in place).  out_dtype: add's,
     out's or dy's."""
     a.check()
+    _no_graph("linear_wgrad8", dy, add, out)
     r = _Rows(dy, dtype, "dy")
     if r.rows != a.rows:
         raise L.OdysseyError(f"dy has {r.rows} rows, the saved activation {a.rows}", L.ERR_SHAPE)

@@ -129,3 +129,26 @@ def test_weights_that_are_not_bytes_are_refused(ody):
         refused(ody, L.ERR_DTYPE, "must be uint8", ody.fp4_linear_dgrad, x[:, :8], w)
         t = ody.QuantizedTensor(torch.from_numpy(w.data), L.Q_NVFP4, 8 * 16)
         refused(ody, L.ERR_DTYPE, "must be uint8", ody.fp4_linear, torch.from_numpy(x), t)
+
+
+def test_products_refuse_to_drop_a_gradient(ody):
+    """The layer's gradients are calls of their own and no graph is recorded:
+    a tensor that asks for one is turned away, unless gradients are off."""
+    from odyssey_b200 import _lib as L
+    import torch
+    n = 32
+    w = ody.QuantizedTensor(torch.zeros(L.quant_bytes(L.Q_NVFP4, n * n), dtype=torch.uint8), L.Q_NVFP4, n * n)
+    a = ody.Activation8(torch.zeros(4, n, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8), 4, n)
+    x, g = torch.ones(4, n), torch.ones(4, n, requires_grad=True)
+    acc = torch.zeros(n, n, requires_grad=True)
+    calls = [(ody.fp4_linear, (g, w), {}), (ody.fp4_linear, (g * 2, w), {}), (ody.fp4_linear, (x, w), {"out": g}),
+             (ody.fp4_linear_dgrad, (g, w), {}), (ody.linear_wgrad8, (g, a), {}), (ody.linear_wgrad8, (x, a), {"add": acc}),
+             (ody.linear_wgrad8, (x, a), {"out": acc})]
+    for fn, args, kw in calls:
+        refused(ody, L.ERR_ARG, "records no gradient", fn, *args, **kw)
+    if not torch.cuda.is_available():  # with gradients off, and for data, the checks let them through
+        for fn, args, kw in calls:
+            with torch.no_grad():
+                refused(ody, L.ERR_CUDA, None, fn, *args, **kw)
+        refused(ody, L.ERR_CUDA, None, ody.fp4_linear, g.detach(), w)
+        refused(ody, L.ERR_CUDA, None, ody.save_activation8, g)
