@@ -214,9 +214,16 @@ def is_torch(x):
 
 def dtype_code(x, dtype=None):
     """F32/F16/BF16 code of an array; numpy bfloat16 data is passed as uint16
-    with dtype='bfloat16'."""
+    with dtype='bfloat16' (which names the elements' type, of their size, and
+    converts nothing)."""
     if dtype is not None:
-        return {"float32": F32, "float16": F16, "bfloat16": BF16, F32: F32, F16: F16, BF16: BF16}[dtype]
+        code = {"float32": F32, "float16": F16, "bfloat16": BF16, F32: F32, F16: F16, BF16: BF16}.get(dtype)
+        if code is None:
+            raise OdysseyError(f"unsupported dtype {dtype}", ERR_DTYPE)
+        size = (x if is_torch(x) else np.asarray(x)).dtype.itemsize
+        if size != (4 if code == F32 else 2):
+            raise OdysseyError(f"dtype {dtype} given for elements of {size} bytes", ERR_DTYPE)
+        return code
     if is_torch(x):
         t = _torch()
         m = {t.float32: F32, t.float16: F16, t.bfloat16: BF16}

@@ -23,6 +23,11 @@ def refused(ody, code, match, fn, *args, **kw):
     assert e.value.code == code
 
 
+def weight(ody, out, inn, kind=7):
+    from odyssey_b200 import _lib as L
+    return ody.QuantizedTensor(np.zeros(L.quant_bytes(kind, out * inn), np.uint8), kind, out * inn)
+
+
 @pytest.mark.parametrize("name", ["fp4_linear", "fp4_linear_dgrad"])
 @pytest.mark.parametrize("torch_weight", [False, True])
 def test_strided_host_weight_lives_until_the_call_is_done(ody, monkeypatch, name, torch_weight):
@@ -152,3 +157,20 @@ def test_products_refuse_to_drop_a_gradient(ody):
                 refused(ody, L.ERR_CUDA, None, fn, *args, **kw)
         refused(ody, L.ERR_CUDA, None, ody.fp4_linear, g.detach(), w)
         refused(ody, L.ERR_CUDA, None, ody.save_activation8, g)
+
+
+def test_a_named_type_has_the_array_s_element_size(ody):
+    """dtype= names the type of raw bits; it does not convert, and a type of
+    another size would read past the array or half of it."""
+    from odyssey_b200 import _lib as L
+    w = weight(ody, 8, 16)
+    f32, f16, u16 = np.ones((2, 16), np.float32), np.ones((2, 16), np.float16), np.ones((2, 16), np.uint16)
+    for x, dtype in ((f32, "bfloat16"), (f32, "float16"), (f16, "float32"), (u16, "float32"), (f32, L.BF16), (f16.astype(float), "float32")):
+        refused(ody, L.ERR_DTYPE, "elements of", ody.fp4_linear, x, w, dtype=dtype)
+        refused(ody, L.ERR_DTYPE, "elements of", ody.save_activation8, x, dtype=dtype)
+        refused(ody, L.ERR_DTYPE, "elements of", ody.quantize, x, L.Q_MXFP4, dtype=dtype)
+        refused(ody, L.ERR_DTYPE, "elements of", ody.check_gradients_finite, x, dtype=dtype)
+    for x, dtype in ((f32, "float64"), (f16, 7)):
+        refused(ody, L.ERR_DTYPE, "unsupported dtype", ody.fp4_linear, x, w, dtype=dtype)
+    for x, dtype in ((f32, "float32"), (f16, "float16"), (u16, "float16"), (u16, "bfloat16"), (u16.view(np.int16), "bfloat16")):
+        assert L.dtype_code(x, dtype) == L.dtype_code(x, L.dtype_code(x, dtype))
