@@ -196,3 +196,55 @@ def test_few_rows_take_no_workspace(ody):
         assert entry(w.kind, w.data.data_ptr(), None, 1.0, out, inn, x.data_ptr(), L.F32, rows, cols, z.data_ptr(), L.F32,
                      others, None, 0, torch.cuda.current_stream().cuda_stream) == L.OK
         assert torch.equal(z, y)
+
+
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def check_gemm(got, terms, reduction, want):
+    """Bound on the tcgen05 path's error with bfloat16 operands, whose products
+    are exact.  One mma adds 16 of them and what the accumulator holds, each
+    cut off at 2^-24 of the largest or below: 17 x 2^-24 of the magnitudes'
+    sum `terms`.  An accumulator takes 32 mma (64 where the result has 16
+    bits), so all of them together lose at most that many times as much of
+    all terms.  The accumulators, one per 512 (1024) of the reduction, and a
+    shared tile's pieces (sqrt(steps) / 2 + 2 at most, steps of 64) are added
+    with rounding; two roundings of the scale and half a step of the result
+    follow."""
+    half = HALF_STEP[got.dtype]
+    mma, chunk = (32, 512) if got.dtype == torch.float32 else (64, 1024)
+    adds = reduction / chunk + 1 + (reduction / 64) ** 0.5 / 2 + 2
+    tol = terms * (mma * 17 * 2.0 ** -24 + adds * 2.0 ** -24 + 2.0 ** -23)
+    R.check(got, want, tol + (np.abs(want) + tol) * half)
+
+
+def pitched(rng, rows, cols, pitch, start=8):
+    """bfloat16 rows whose begin and pitch are multiples of 16 bytes, NaN all around."""
+    buf = torch.full((rows + 2, pitch), float("nan"), dtype=torch.bfloat16, device="cuda")
+    view = buf[1:rows + 1, start:start + cols]
+    view.copy_(torch.from_numpy(rng.standard_normal((rows, cols)).astype(np.float32)))
+    assert view.data_ptr() % 16 == 0 and pitch % 8 == 0 and pitch > start + cols
+    return view
+
+
+@pytest.mark.parametrize("rows,out,inn", [(700, 1100, 1030), (1025, 769, 1568), (300, 2500, 2000), (257, 3001, 4112)])
+@pytest.mark.parametrize("out_dtype", ["bfloat16", "float32"])
+def test_rows_read_in_place_at_a_pitch(ody, rows, out, inn, out_dtype):
+    """bfloat16 rows that the tensor map reads where they lie, wider apart than
+    their columns (whole and broken eights and tiles): nothing of what lies
+    around them reaches a result."""
+    from odyssey_b200 import _lib as L
+    rng = np.random.default_rng(rows)
+    of = L.lib().ody_linear_workspace_of
+    assert all(of(op, 6 * (op < 2), rows, out, inn, L.BF16) > 0 for op in range(3))  # none: another path
+    q = R.random_weight(rng, R.MXFP4, out, inn)
+    w, w64 = ody.QuantizedTensor(torch.from_numpy(q).cuda(), R.MXFP4, out * inn), R.weight(R.MXFP4, q, out, inn)
+    for fn, cols, m in ((ody.fp4_linear, inn, w64.T), (ody.fp4_linear_dgrad, out, w64)):
+        x = pitched(rng, rows, cols, (cols + 31) // 8 * 8)
+        x64 = R.to64(x)
+        check_gemm(fn(x, w, out_dtype=out_dtype), np.abs(x64) @ np.abs(m), cols, x64 @ m)
+        assert torch.equal(fn(x, w, out_dtype=out_dtype), fn(x.contiguous(), w, out_dtype=out_dtype))
+    a = ody.save_activation8(pitched(rng, rows, inn, (inn + 31) // 8 * 8))
+    dy = pitched(rng, rows, out, (out + 31) // 8 * 8, 16)
+    d64, x64 = R.to64(dy), R.to64(ody.load_activation8(a, "float32"))
+    check_gemm(ody.linear_wgrad8(dy, a, out_dtype=out_dtype), np.abs(d64.T) @ np.abs(x64), rows, d64.T @ x64)
