@@ -12,22 +12,12 @@ struct W4 {
   static constexpr bool MX = KIND == Q_MXFP4 || KIND == Q_MXFP4_OCP;
   static constexpr int BE = MX ? 32 : 16;  // elements per block
   static constexpr int SB = MX ? 17 : 9;   // bytes per block
-
-  // code times scale; exact in float32 and, for finite scales, in bfloat16:
-  // two bits of value times at most four of scale.  Code 1 is 0.5 in the OCP
-  // kind and 0 in the others, and their zero is not multiplied by the scale.
-  static __device__ __forceinline__ float value(uint32_t code, float sf) {
-    if (KIND == Q_MXFP4_OCP) {
-      const uint32_t e = (code >> 1) & 3u, m = code & 1u;
-      const float un = e ? (m ? 1.5f : 1.0f) * (float)(1u << (e - 1)) : 0.5f * (float)m;
-      const float r = __fmul_rn(un, sf);
-      return code & 8u ? -r : r;
-    }
-    return fp4_decode(code, sf);
-  }
 };
 
 // ---- eight weights at once, as bfloat16 pairs -------------------------------
+// Code times scale is exact in bfloat16 for finite scales: two bits of value
+// times at most four of scale.  Code 1 is 0.5 in the OCP kind and 0 in the
+// others.
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));

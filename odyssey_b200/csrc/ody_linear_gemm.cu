@@ -209,7 +209,6 @@ constexpr long long kWaitCycles = 4000000000ll;
 // set when a bounded wait ran out; read and cleared by gemm_wait_error
 __device__ unsigned g_gemm_err;
 
-__device__ __forceinline__ uint32_t sptr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -270,9 +269,6 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Shared-memory descriptor of a 128-byte-swizzled operand: K-major, rows of
 // 64 k at 128 bytes, eight rows every 1024 bytes; MN-major, the same rows are
@@ -423,8 +419,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
   __shared__ __align__(8) uint64_t bars[2 * kStages + 5];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
-  const uint32_t smem = (sptr(dyn) + 1023u) & ~1023u;
-  const uint32_t full = sptr(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16,
+  const uint32_t smem = (srow(dyn) + 1023u) & ~1023u;
+  const uint32_t full = srow(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16,
                  drain = tempty + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -437,12 +433,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sptr(&tmem_base)) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(srow(&tmem_base)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  cluster_sync();
+  cluster_barrier();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_base;
   let_next_start();
@@ -527,7 +523,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     const uint32_t done = in_cta(tempty, 0);
     // a warp goes on, or stops after a wait that ran out, as one
     const auto together = [](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
-    float* buf32 = reinterpret_cast<float*>(dyn + (smem - sptr(dyn)) + kStages * kStageBytes) + (warp - 4) * 32 * 32;
+    float* buf32 = reinterpret_cast<float*>(dyn + (smem - srow(dyn)) + kStages * kStageBytes) + (warp - 4) * 32 * 32;
     const float scale = out_scale(g.o);
     constexpr int ES = DT == DT_F32 ? 4 : 2;
     int chunk = 0;
@@ -599,7 +595,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     }
   }
   __syncwarp();
-  cluster_sync();
+  cluster_barrier();
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
@@ -624,7 +620,7 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs g) {
     const int64_t m = (int64_t)tm * kBM + r;
     if (m >= g.M) return;
     const float* s = g.partial + r * kBN + c;
-    float4 v = *reinterpret_cast<const float4*>(s + (int64_t)(2 * first + ((int64_t)first * g.deal <= t0)) * kBM * kBN);
+    float4 v = *reinterpret_cast<const float4*>(s + (int64_t)(2 * first + 1) * kBM * kBN);  // the tile's begin
 #pragma unroll 4
     for (int q = first + 1; q <= last; q++) {
       const float4 f = *reinterpret_cast<const float4*>(s + (int64_t)(2 * q) * kBM * kBN);  // begins inside the tile
@@ -669,8 +665,8 @@ __global__ void wait_selftest_kernel(long long limit) {
   __shared__ __align__(8) uint64_t bar;
   __shared__ int abort_flag;
   abort_flag = 0;
-  mbar_init(sptr(&bar), 1);
-  mbar_wait(sptr(&bar), 0, &abort_flag, limit);
+  mbar_init(srow(&bar), 1);
+  mbar_wait(srow(&bar), 0, &abort_flag, limit);
 }
 
 // ---------------------------------------------------------------------------
