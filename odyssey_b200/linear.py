@@ -52,17 +52,23 @@ def _code(dtype):
     return c
 
 
-def _check_bytes(b, what):
-    if (b if L.is_torch(b) else np.asarray(b)).dtype.itemsize != 1:
+def _count_bytes(b, what):
+    """The bytes of a buffer of bytes."""
+    if L.is_torch(b):
+        n, size = b.numel(), b.element_size()
+    else:
+        b = np.asarray(b)
+        n, size = b.size, b.itemsize
+    if size != 1:
         raise L.OdysseyError(f"{what} must be uint8", L.ERR_DTYPE)
+    return n
 
 
-def _no_graph(name, *buffers):
-    """Refuses tensors whose gradient would be lost: nothing here records one."""
-    for b in buffers:
-        if getattr(b, "requires_grad", False) and L._torch().is_grad_enabled():
-            raise L.OdysseyError(f"{name} records no gradient: detach its tensors or call it under torch.no_grad() "
-                                 "(the layer's gradients are fp4_linear_dgrad and linear_wgrad8)", L.ERR_ARG)
+def _no_graph(name, tensor):
+    """Refuses a tensor whose gradient would be lost: nothing here records one."""
+    if getattr(tensor, "requires_grad", False) and L._torch().is_grad_enabled():
+        raise L.OdysseyError(f"{name} records no gradient: detach its tensors or call it under torch.no_grad() "
+                             "(the layer's gradients are fp4_linear_dgrad and linear_wgrad8)", L.ERR_ARG)
 
 
 @dataclass
@@ -85,15 +91,14 @@ class Activation8:
         if self.rows <= 0 or self.cols <= 0:
             raise L.OdysseyError("cannot save an empty activation", L.ERR_SHAPE)
         for b, n in ((self.codes, self.rows * g * 32), (self.scales, self.rows * g)):
-            if L.numel(b) != n:
+            if _count_bytes(b, "codes and scales") != n:
                 raise L.OdysseyError("codes and scales do not have the bytes of the activation's rows and columns",
                                      L.ERR_SHAPE)
-            _check_bytes(b, "codes and scales")
 
 
 class _Rows:
     """An array as rows of its last axis: the code of its type and its pitch."""
-    __slots__ = ("a", "code", "rows", "cols", "ld", "cuda", "ptr", "lead")
+    __slots__ = ("a", "code", "rows", "cols", "ld", "cuda", "ptr", "lead", "grad")
 
     def __init__(self, x, dtype, what):
         if L.is_torch(x):
@@ -103,7 +108,7 @@ class _Rows:
             shape = x.shape
             if len(shape) == 0 or x.numel() == 0:
                 raise L.OdysseyError(f"{what} is empty", L.ERR_SHAPE)
-            self.cuda = x.is_cuda
+            self.cuda, self.grad = x.is_cuda, x.requires_grad
             if len(shape) != 2:
                 x = x.reshape(-1, shape[-1])
             rows, cols = x.shape
@@ -120,7 +125,7 @@ class _Rows:
             x = np.ascontiguousarray(x)
             if len(shape) == 0 or x.size == 0:
                 raise L.OdysseyError(f"{what} is empty", L.ERR_SHAPE)
-            self.cuda = False
+            self.cuda = self.grad = False
             x = x.reshape(-1, shape[-1])
             rows, cols = x.shape
             self.ld = cols
@@ -138,7 +143,7 @@ class _Place:
 def _same_place(x, *others):
     """Buffers of one call live on one device (or all on the host)."""
     for o in others:
-        t = L.is_torch(o) and o.is_cuda
+        t = getattr(o, "is_cuda", False)
         if t != x.cuda or (t and o.get_device() != x.a.get_device()):
             raise L.OdysseyError("the buffers of a call must be on one device", L.ERR_ARG)
 
@@ -207,13 +212,15 @@ def _weight(name, op, kind, numel, features):
 def _product(name, op, x, w, out, out_dtype, dtype, what):
     if not isinstance(w, QuantizedTensor) or w.kind not in _BLOCK:
         raise L.OdysseyError(f"{name} takes a weight of the 4-bit kinds", L.ERR_ARG)
-    _no_graph(name, x, out, w.tensor_scale)
     r = _Rows(x, dtype, what)
+    if r.grad:
+        _no_graph(name, x)
+    if out is not None:
+        _no_graph(name, out)
     other, nout, nin, need = _weight(name, op, w.kind, w.original_numel, r.cols)
     data = w.data
-    if L.numel(data) != need:
+    if _count_bytes(data, "the weight's buffer") != need:
         raise L.OdysseyError(f"quantised buffer has {L.numel(data)} bytes, expected {need}", L.ERR_SHAPE)
-    _check_bytes(data, "the weight's buffer")
     code = r.code if out_dtype is None else _code(out_dtype)
     y = _out(r, out, (*r.lead, other), code, "out")
     lib = L.lib()
@@ -228,6 +235,7 @@ def _product(name, op, x, w, out, out_dtype, dtype, what):
     if w.kind == L.Q_NVFP4_TENSOR:
         if L.is_torch(w.tensor_scale):  # a device float: read by the kernel, no synchronisation
             _same_place(r, w.tensor_scale)
+            _no_graph(name, w.tensor_scale)
             if w.tensor_scale.numel() != 1 or w.tensor_scale.dtype != L._torch().float32:
                 raise L.OdysseyError("the tensor scale must be one float32", L.ERR_DTYPE)
             ts = w.tensor_scale.data_ptr()
@@ -301,8 +309,10 @@ def linear_wgrad8(dy, a, add=None, alpha=1.0, out=None, out_dtype=None, dtype=No
     result's type; it may be `out` (accumulation in place).  out_dtype: add's,
     out's or dy's."""
     a.check()
-    _no_graph("linear_wgrad8", dy, add, out)
     r = _Rows(dy, dtype, "dy")
+    for b in (dy, add, out):
+        if b is not None:
+            _no_graph("linear_wgrad8", b)
     if r.rows != a.rows:
         raise L.OdysseyError(f"dy has {r.rows} rows, the saved activation {a.rows}", L.ERR_SHAPE)
     _same_place(r, a.codes, a.scales)
