@@ -2,22 +2,23 @@
 libodyssey_mp.so (extensions; the reference's linear layer works on float
 tensors).
 
-    y  = fp4_linear(x, w)             y  = x W^T    W in 4 bits, as the step leaves it
+    y  = fp4_linear(x, w)             y  = x W^T    W in 4 bits, in the step's bytes
     dx = fp4_linear_dgrad(dy, w)      dx = dy W
     a  = save_activation8(x)          x kept in 8 bits for the backward pass
     x' = load_activation8(a)
     dW = linear_wgrad8(dy, a)         dW = dy^T x'
 
 Weights are QuantizedTensors of the 4-bit kinds (to_mxfp4, to_nvfp4,
-to_nvfp4_tensor_scaled, to_mxfp4_ocp, MixedPrecisionStep.get_quant), read
-where they lie.  Activations and gradients are float32, float16 or bfloat16
-arrays whose last axis is the feature axis; leading axes are tokens.  CUDA
-tensors run on torch's current stream of their device without waiting, host
-arrays (numpy, or torch on the CPU; bfloat16 numpy data as uint16 with
-dtype='bfloat16') are staged and the call returns when done.  A result may not
-share memory with an operand (linear_wgrad8's add=out apart); such a call is
-refused.  The gradients are calls of their own: no autograd graph is recorded,
-and a product of a tensor that requires one is refused while gradients are on.
+to_nvfp4_tensor_scaled, to_mxfp4_ocp, or the copy that
+MixedPrecisionStep.get_quant makes of the step's), read in place. Activations
+and gradients are float32, float16 or bfloat16 arrays whose last axis is the
+feature axis; leading axes are tokens. CUDA tensors run on torch's current
+stream of their device without waiting, host arrays (numpy, or torch on the
+CPU; bfloat16 numpy data as uint16 with dtype='bfloat16') are staged and the
+call returns when done. A result may not share memory with an operand
+(linear_wgrad8's add=out apart); such a call is refused. The gradients are
+calls of their own: no autograd graph is recorded, and a product of a tensor
+that requires one is refused while gradients are on.
 """
 import ctypes as C
 from dataclasses import dataclass
