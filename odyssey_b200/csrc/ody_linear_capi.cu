@@ -76,9 +76,10 @@ struct Span {
 };
 Span flat(const void* p, int64_t bytes) { return {p, 1, bytes, bytes}; }
 
-// Whether two buffers share a byte.  Rows may interleave (columns of one wide
-// buffer), so where the extents meet, each row of the one with fewer rows is
-// compared with the first row of the other that ends behind its begin.
+// Whether two buffers share a byte.  Rows may interleave: at one pitch
+// (columns of one wide buffer) their places in it tell; else, where the
+// extents meet, each row of the buffer with fewer is compared with the first
+// row of the other that ends behind its begin.
 bool meet(const Span& u, const Span& v) {
   if (!u.p || !v.p) return false;
   using Wide = __int128;  // a pitch times a number of rows may pass 64 bits
@@ -86,6 +87,10 @@ bool meet(const Span& u, const Span& v) {
   const Wide a = (Wide)(uintptr_t)x.p, b = (Wide)(uintptr_t)y.p;
   const Wide a_end = a + (Wide)(x.n - 1) * x.pitch + x.bytes, b_end = b + (Wide)(y.n - 1) * y.pitch + y.bytes;
   if (a_end <= b || b_end <= a) return false;
+  if (x.pitch == y.pitch) {
+    const Wide d = b >= a ? (b - a) % x.pitch : x.pitch - 1 - (a - b - 1) % x.pitch;  // y's place in x's pitch
+    if (d >= x.bytes && d + y.bytes <= x.pitch) return false;
+  }
   for (int64_t i = 0; i < x.n; i++) {
     const Wide s = a + (Wide)i * x.pitch, e = s + x.bytes;
     const Wide j = s - b < y.bytes ? 0 : (s - b - y.bytes) / y.pitch + 1;
