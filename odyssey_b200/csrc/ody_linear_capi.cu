@@ -282,8 +282,8 @@ extern "C" int ody_act8_load(int32_t fmt, const uint8_t* codes, const uint8_t* s
 extern "C" int64_t ody_linear_workspace_of(int32_t op, int32_t kind, int64_t rows, int64_t out, int64_t in,
                                            int32_t act_dtype) {
   LinearArgs a{};
-  if (op < LIN_FORWARD || op > LIN_WGRAD || (op != LIN_WGRAD && !is_w4(kind)) || rows <= 0 || out <= 0 || in <= 0 || rows > kMaxDim || out > kMaxDim ||
-      in > kMaxDim || act_dtype < DT_F32 || act_dtype > DT_BF16)
+  if (op < LIN_FORWARD || op > LIN_WGRAD || (op != LIN_WGRAD && !is_w4(kind)) || rows <= 0 || out <= 0 || in <= 0 ||
+      rows > kMaxDim || out > kMaxDim || in > kMaxDim || act_dtype < DT_F32 || act_dtype > DT_BF16)
     return -1;
   a.op = op;
   a.rows = rows, a.out = out, a.in = in;
